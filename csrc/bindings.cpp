@@ -9,6 +9,7 @@
 
 #include "kernels/chunk_rows.h"
 #include "kernels/launch.h"
+#include "kernels/rope_axes.h"
 
 namespace {
 
@@ -97,14 +98,150 @@ bool kv_is_fp8(const Tensor& k_cache, const Tensor& v_cache, at::ScalarType act)
   return false;
 }
 
+// positions [T], or [A, T] with the pairs of a head that each axis turns (rope_axes.h)
+kgc::RopeAxes rope_axes(const Tensor& positions, at::OptionalIntArrayRef sections, const Tensor& cos_sin, int64_t T,
+                        int64_t d, bool use_rope) {
+  kgc::RopeAxes ax{};
+  TORCH_CHECK(positions.scalar_type() == at::kLong, "positions int64");
+  TORCH_CHECK(cos_sin.dim() == 2 && cos_sin.size(0) < ((int64_t)1 << 31), "cos_sin fp32 [max_pos, d]");
+  ax.rows = (int)cos_sin.size(0);
+  if (!sections.has_value()) {
+    TORCH_CHECK(positions.numel() == T, "positions int64 [T]");
+    return ax;
+  }
+  const int64_t A = (int64_t)sections->size();
+  TORCH_CHECK(use_rope && A >= 1 && A <= kgc::ROPE_MAX_AXES, "kgc.rope_kv_write: 1 to ", kgc::ROPE_MAX_AXES,
+              " sections of a rotated head");
+  TORCH_CHECK(positions.dim() == 2 && positions.size(0) == A && positions.size(1) == T &&
+              (T <= 1 || positions.stride(1) == 1), "kgc.rope_kv_write: positions int64 [sections, T] with dense rows");
+  TORCH_CHECK(ax.rows > 0, "kgc.rope_kv_write: an empty cos_sin");
+  int64_t end = 0;
+  for (int64_t a = 0; a < A; ++a) {
+    TORCH_CHECK((*sections)[a] >= 0 && (*sections)[a] <= d / 2, "kgc.rope_kv_write: a section is 0 to d / 2 pairs");
+    ax.end[a] = (int)(end += (*sections)[a]);
+  }
+  TORCH_CHECK(end == d / 2, "kgc.rope_kv_write: sections of ", end, " pairs in all; a head has ", d / 2);
+  ax.n = (int)A;
+  ax.stride = positions.stride(0);
+  return ax;
+}
+
+// ---- the cache in 4 bits: uint8 [nb, nkv, bs, d / 2 + d / 32], a head's page as csrc/kernels/kv4.h has it
+void check_kv4(const Tensor& k_cache, const Tensor& v_cache, int64_t nkv, int64_t d, const Tensor& with) {
+  TORCH_CHECK(k_cache.scalar_type() == at::kByte && v_cache.scalar_type() == at::kByte,
+              "k/v cache dtype mismatch: a 4-bit cache is uint8, keys and values");
+  TORCH_CHECK(d == 64 || d == 128, "4-bit cache: head_dim must be 64 or 128");
+  TORCH_CHECK(k_cache.dim() == 4 && v_cache.dim() == 4 && k_cache.is_contiguous() && v_cache.is_contiguous() &&
+              k_cache.sizes() == v_cache.sizes() && k_cache.size(1) == nkv && k_cache.size(3) == d / 2 + d / 32,
+              "4-bit cache: k_cache and v_cache uint8 [nb, ", nkv, ", bs, ", d / 2 + d / 32, "] contiguous");
+  TORCH_CHECK(k_cache.size(2) >= 16, "block_size must be >= 16");
+  log2_exact(k_cache.size(2), "block_size");
+  TORCH_CHECK(k_cache.size(0) < ((int64_t)1 << 31) && k_cache.size(2) <= 65536, "4-bit cache: pages");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(k_cache.data_ptr()) % 16 == 0 &&
+              reinterpret_cast<uintptr_t>(v_cache.data_ptr()) % 16 == 0, "4-bit cache: 16-byte aligned pages");
+  check_same_dev(with, k_cache, "k_cache");
+  check_same_dev(with, v_cache, "v_cache");
+}
+void no_kv4_scale(double k_scale, double v_scale) {
+  TORCH_CHECK(k_scale == 1.0 && v_scale == 1.0, "a 4-bit cache has its own scales: k_scale = v_scale = 1");
+}
+void aligned16(const Tensor& t, const char* name) {
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "kgc: ", name, " must be 16-byte aligned");
+}
+
+void kv4_write(const Tensor& qkv, int64_t stride, int64_t S, int64_t slice_stride, const Tensor& positions,
+               const Tensor& cos_sin, const Tensor& q_out, const Tensor& k_cache, const Tensor& v_cache,
+               const Tensor& slot_mapping, const std::optional<Tensor>& q_norm_w, const std::optional<Tensor>& k_norm_w,
+               int64_t T, int64_t nq, int64_t nkv, int64_t d, double eps, bool use_rope, double k_scale, double v_scale,
+               const kgc::RopeAxes& ax) {
+  check_kv4(k_cache, v_cache, nkv, d, qkv);
+  no_kv4_scale(k_scale, v_scale);
+  TORCH_CHECK(!use_rope || ax.rows > 0, "kgc.rope_kv_write: an empty cos_sin");
+  TORCH_CHECK(slot_mapping.is_contiguous() && (ax.n || positions.is_contiguous()), "positions, slot_mapping contiguous");
+  TORCH_CHECK(T * (nq + 2 * nkv) * (d / 16) < ((int64_t)1 << 31) * 256 && T < ((int64_t)1 << 31), "kgc.rope_kv_write: rows");
+  aligned16(qkv, "qkv");
+  aligned16(q_out, "q_out");
+  aligned16(cos_sin, "cos_sin");
+  kgc::Kv4Write w{};
+  if (q_norm_w.has_value()) {
+    TORCH_CHECK(k_norm_w.has_value() && q_norm_w->numel() == d && k_norm_w->numel() == d, "qk norm weights");
+    for (const Tensor* t : {&*q_norm_w, &*k_norm_w}) {
+      TORCH_CHECK(t->scalar_type() == q_out.scalar_type() && t->is_contiguous(), "qk norm weights in q's dtype");
+      check_same_dev(qkv, *t, "qk norm weights");
+      aligned16(*t, "qk norm weights");
+    }
+    w.q_norm_w = q_norm_w->data_ptr();
+    w.k_norm_w = k_norm_w->data_ptr();
+  }
+  w.qkv = qkv.data_ptr();
+  w.qkv_stride = stride;
+  w.slice_stride = slice_stride;
+  w.S = (int)S;
+  w.positions = positions.data_ptr<int64_t>();
+  w.cos_sin = cos_sin.data_ptr<float>();
+  w.q_out = q_out.data_ptr();
+  w.k_cache = k_cache.data_ptr();
+  w.v_cache = v_cache.data_ptr();
+  w.slots = slot_mapping.data_ptr<int64_t>();
+  w.T = T;
+  w.nq = (int)nq;
+  w.nkv = (int)nkv;
+  w.d = (int)d;
+  w.bs = (int)k_cache.size(2);
+  w.num_blocks = (int)k_cache.size(0);
+  w.eps = (float)eps;
+  w.use_rope = use_rope;
+  kgc::launch_kv4_write(dt_code(q_out), w, ax, stream());
+}
+
+void kv4_read(Tensor out, Tensor cache, Tensor slots) {
+  check_gpu(cache, "cache");
+  c10::hip::HIPGuardMasqueradingAsCUDA g(cache.device());
+  TORCH_CHECK(out.dim() == 3 && out.is_contiguous() &&
+              (out.scalar_type() == at::kBFloat16 || out.scalar_type() == at::kHalf),
+              "kgc.kv4_read: out bf16 / fp16 [n, nkv, d] contiguous");
+  check_kv4(cache, cache, out.size(1), out.size(2), out);
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.numel() == out.size(0),
+              "kgc.kv4_read: slots int64 [n]");
+  check_same_dev(out, slots, "slots");
+  aligned16(out, "out");
+  TORCH_CHECK(out.numel() / 8 < ((int64_t)1 << 31) * 256, "kgc.kv4_read: rows");
+  kgc::launch_kv4_read(dt_code(out), out.data_ptr(), cache.data_ptr(), slots.data_ptr<int64_t>(), out.size(0),
+                       (int)out.size(1), (int)out.size(2), (int)cache.size(2), (int)cache.size(0), stream());
+}
+
+// what both attention forms over a 4-bit cache ask for
+void check_kv4_attention(const Tensor& q, const Tensor& out, const Tensor& k_cache, const Tensor& v_cache,
+                         const Tensor& block_tables, double k_scale, double v_scale) {
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "attention kernels take bf16/f16");
+  TORCH_CHECK(k_cache.dim() == 4 && k_cache.size(1) >= 1, "4-bit cache: uint8 [nb, nkv, bs, d / 2 + d / 32]");
+  const int64_t nq = q.size(1), nkv = k_cache.size(1);
+  check_kv4(k_cache, v_cache, nkv, q.size(2), q);
+  no_kv4_scale(k_scale, v_scale);
+  TORCH_CHECK(nq % nkv == 0 && nq / nkv <= 16, "GQA group must be <= 16");
+  TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out");
+  check_same_dev(q, out, "out");
+  TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
+              block_tables.size(1) >= 1 && block_tables.size(1) * k_cache.size(2) < ((int64_t)1 << 31),
+              "block_tables int32 [rows, max_blocks] contiguous");
+  check_same_dev(q, block_tables, "block_tables");
+  aligned16(q, "q");
+  aligned16(out, "out");
+}
+
 // qkv: [T, >= (nq+2nkv)*d] in q_out's dtype, or the K9m split-K slices fp32 [S, T, N]
 void rope_kv_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor q_out, Tensor k_cache,
                    Tensor v_cache, Tensor slot_mapping, std::optional<Tensor> q_norm_w,
                    std::optional<Tensor> k_norm_w, int64_t nq, int64_t nkv, int64_t d,
-                   double eps, bool use_rope, double k_scale, double v_scale) {
+                   double eps, bool use_rope, double k_scale, double v_scale, at::OptionalIntArrayRef sections) {
   check_gpu(qkv, "qkv");
   c10::hip::HIPGuardMasqueradingAsCUDA g(qkv.device());
   TORCH_CHECK(d % 16 == 0 && d <= 256, "kgc.rope_kv_write: head_dim");
+  const bool kv4 = k_cache.scalar_type() == at::kByte || v_cache.scalar_type() == at::kByte;
+  // (an op of its own case: what else it reads was always this op's caller's to give)
+  if (kv4 || sections.has_value())
+    for (const Tensor* t : {&positions, &cos_sin, &q_out, &k_cache, &v_cache, &slot_mapping})
+      check_same_dev(qkv, *t, "rope_kv_write operand");
   const bool slices = qkv.dim() == 3;
   const int64_t T = slices ? qkv.size(1) : qkv.size(0);
   int64_t S = 0, ss = 0, stride;
@@ -123,7 +260,7 @@ void rope_kv_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor q_out, T
   }
   TORCH_CHECK(q_out.scalar_type() == at::kBFloat16 || q_out.scalar_type() == at::kHalf,
               "q_out bf16 / fp16");
-  TORCH_CHECK(positions.scalar_type() == at::kLong && positions.numel() == T, "positions int64 [T]");
+  const kgc::RopeAxes ax = rope_axes(positions, sections, cos_sin, T, d, use_rope);
   TORCH_CHECK(slot_mapping.scalar_type() == at::kLong && slot_mapping.numel() == T, "slot_mapping int64 [T]");
   TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() && cos_sin.size(1) == d,
               "cos_sin fp32 [max_pos, d]");
@@ -131,6 +268,12 @@ void rope_kv_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor q_out, T
   const bool kv_only = q_out.numel() == 0;
   TORCH_CHECK(kv_only || (q_out.is_contiguous() && q_out.numel() == T * nq * d),
               "q_out [T, nq, d] (or empty: k / v only)");
+  if (ax.n || kv4) TORCH_CHECK(!kv_only || T == 0 || nq == 0, "kgc.rope_kv_write: 4-bit caches and sections write q too");
+  if (kv4) {
+    kv4_write(qkv, stride, S, ss, positions, cos_sin, q_out, k_cache, v_cache, slot_mapping, q_norm_w, k_norm_w, T, nq,
+              nkv, d, eps, use_rope, k_scale, v_scale, ax);
+    return;
+  }
   TORCH_CHECK(k_cache.is_contiguous() && v_cache.is_contiguous() && k_cache.dim() == 4 &&
               v_cache.dim() == 5 && k_cache.size(1) == nkv && k_cache.size(3) == d &&
               v_cache.size(3) == d && v_cache.size(4) == 8 &&
@@ -150,7 +293,7 @@ void rope_kv_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor q_out, T
                             v_cache.data_ptr(), slot_mapping.data_ptr<int64_t>(), qn, kn,
                             (int)T, (int)nq, (int)nkv,
                             (int)d, (int)k_cache.size(2), (float)eps, use_rope, kv8,
-                            (float)k_scale, (float)v_scale, (int)k_cache.size(0), stream());
+                            (float)k_scale, (float)v_scale, (int)k_cache.size(0), ax, stream());
 }
 
 void check_kv(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, int64_t nq) {
@@ -188,6 +331,36 @@ void paged_decode(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor b
   check_gpu(q, "q");
   c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
   TORCH_CHECK(q.dim() == 3 && q.is_contiguous(), "q [B, nq, d] contiguous");
+  if (k_cache.scalar_type() == at::kByte) {
+    check_kv4_attention(q, out, k_cache, v_cache, block_tables, k_scale, v_scale);
+    const int64_t B = q.size(0), nq = q.size(1), d = q.size(2);
+    TORCH_CHECK(B < ((int64_t)1 << 31) && k_cache.size(1) <= 65535 && nq <= 65535, "grid");
+    TORCH_CHECK(block_tables.size(0) >= B, "block_tables int32 [B, max_blocks]");
+    TORCH_CHECK(ctx_lens.scalar_type() == at::kInt && ctx_lens.is_contiguous() && ctx_lens.numel() >= B, "ctx_lens int32 [B]");
+    check_same_dev(q, ctx_lens, "ctx_lens");
+    check_partials(max_logits, exp_sums, tmp_out, B, nq, d, Z, "kgc.paged_decode");
+    check_same_dev(q, tmp_out, "partials");
+    kgc::Kv4Decode a{};
+    a.q = q.data_ptr();
+    a.k_cache = k_cache.data_ptr();
+    a.v_cache = v_cache.data_ptr();
+    a.out = out.data_ptr();
+    a.block_tables = block_tables.data_ptr<int>();
+    a.ctx_lens = ctx_lens.data_ptr<int>();
+    a.max_logits = max_logits.data_ptr<float>();
+    a.exp_sums = exp_sums.data_ptr<float>();
+    a.tmp_out = tmp_out.data_ptr<float>();
+    a.bt_stride = (int)block_tables.size(1);
+    a.B = (int)B;
+    a.nq = (int)nq;
+    a.nkv = (int)k_cache.size(1);
+    a.D = (int)d;
+    a.bs_log2 = log2_exact(k_cache.size(2), "block_size");
+    a.Z = (int)Z;
+    a.num_blocks = (int)k_cache.size(0);
+    kgc::launch_kv4_decode(dt_code(q), a, (float)scale, stream());
+    return;
+  }
   const int64_t B = q.size(0), nq = q.size(1), d = q.size(2);
   check_kv(q, k_cache, v_cache, nq);
   TORCH_CHECK(k_cache.size(3) == d, "head_dim mismatch");
@@ -289,6 +462,36 @@ void prefill_attention(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Ten
   check_gpu(q, "q");
   c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
   TORCH_CHECK(q.dim() == 3 && q.is_contiguous(), "q [T, nq, d] contiguous");
+  if (k_cache.scalar_type() == at::kByte) {
+    check_kv4_attention(q, out, k_cache, v_cache, block_tables, k_scale, v_scale);
+    const int64_t P = block_tables.size(0);
+    TORCH_CHECK(query_start_loc.scalar_type() == at::kInt && query_start_loc.is_contiguous() &&
+                query_start_loc.numel() == P + 1, "query_start_loc");
+    TORCH_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.is_contiguous() && seq_lens.numel() >= P, "seq_lens int32");
+    TORCH_CHECK(work_seq.scalar_type() == at::kInt && work_mblk.scalar_type() == at::kInt && work_seq.is_contiguous() &&
+                work_mblk.is_contiguous() && work_seq.numel() == work_mblk.numel(), "work list");
+    for (const Tensor* t : {&query_start_loc, &seq_lens, &work_seq, &work_mblk}) check_same_dev(q, *t, "prefill operand");
+    TORCH_CHECK(work_seq.numel() <= 2147483647 && q.size(1) <= 65535, "grid");
+    kgc::Kv4Prefill a{};
+    a.q = q.data_ptr();
+    a.k_cache = k_cache.data_ptr();
+    a.v_cache = v_cache.data_ptr();
+    a.out = out.data_ptr();
+    a.block_tables = block_tables.data_ptr<int>();
+    a.query_start_loc = query_start_loc.data_ptr<int>();
+    a.seq_lens = seq_lens.data_ptr<int>();
+    a.work_seq = work_seq.data_ptr<int>();
+    a.work_mblk = work_mblk.data_ptr<int>();
+    a.bt_stride = (int)block_tables.size(1);
+    a.n_work = (int)work_seq.numel();
+    a.nq = (int)q.size(1);
+    a.nkv = (int)k_cache.size(1);
+    a.D = (int)q.size(2);
+    a.bs_log2 = log2_exact(k_cache.size(2), "block_size");
+    a.num_blocks = (int)k_cache.size(0);
+    kgc::launch_kv4_prefill(dt_code(q), a, (float)scale, stream());
+    return;
+  }
   const int64_t nq = q.size(1), d = q.size(2);
   check_kv(q, k_cache, v_cache, nq);
   TORCH_CHECK(k_cache.size(3) == d, "head_dim mismatch");
@@ -1026,8 +1229,9 @@ void u32_clear_async(int64_t addr) {
 
 // debug builds: OR of the K1/K2/K3 bounds-check error words (read and cleared)
 int64_t debug_errors() {
-  return (int64_t)(kgc::dbg_err_attention_decode() | (kgc::dbg_err_attention_prefill() << 1) |
-                   (kgc::dbg_err_rope_cache() << 2));
+  return (int64_t)(kgc::dbg_err_attention_decode() | kgc::dbg_err_kv4_decode() |
+                   ((kgc::dbg_err_attention_prefill() | kgc::dbg_err_kv4_prefill()) << 1) |
+                   ((kgc::dbg_err_rope_cache() | kgc::dbg_err_kv4_cache()) << 2));
 }
 
 bool debug_build() {
@@ -2778,7 +2982,8 @@ TORCH_LIBRARY(kgc, m) {
   m.def("rope_kv_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor(a!) q_out, "
         "Tensor(b!) k_cache, Tensor(c!) v_cache, Tensor slot_mapping, Tensor? q_norm_w, "
         "Tensor? k_norm_w, int nq, int nkv, int d, float eps, bool use_rope, float k_scale=1.0, "
-        "float v_scale=1.0) -> ()");
+        "float v_scale=1.0, int[]? sections=None) -> ()");
+  m.def("kv4_read(Tensor(a!) out, Tensor cache, Tensor slots) -> ()");
   m.def("paged_decode(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, "
         "Tensor block_tables, Tensor ctx_lens, Tensor(b!) max_logits, Tensor(c!) exp_sums, "
         "Tensor(d!) tmp_out, int Z, float scale, float k_scale=1.0, "
@@ -2928,6 +3133,7 @@ TORCH_LIBRARY_IMPL(kgc, CUDA, m) {
   m.impl("layer_norm", &layer_norm);
   m.impl("silu_mul", &silu_mul);
   m.impl("rope_kv_write", &rope_kv_write);
+  m.impl("kv4_read", &kv4_read);
   m.impl("paged_decode", &paged_decode);
   m.impl("paged_decode_rope", &paged_decode_rope);
   m.impl("prefill_attention", &prefill_attention);

@@ -1094,6 +1094,22 @@ void launch_paged_decode_rope(int dtype, const DecodeRope& rp, void* out, void* 
                       k_scale, v_scale, num_blocks, rp, s);
 }
 
+void launch_paged_decode_merge(int dtype, void* out, const float* max_logits, const float* exp_sums, const float* tmp_out,
+                               const int* ctx_lens, int B, int nq, int D, int Z, int ctx_cap, const DecodeLeast& least,
+                               hipStream_t s) {
+#define KGC_MERGE(TT, DD)                                                                                   \
+  paged_decode_reduce_kernel<TT, DD, true><<<dim3(B, nq), 64, 0, s>>>((TT*)out, max_logits, exp_sums, tmp_out, \
+                                                                      ctx_lens, nq, Z, Z, ctx_cap, least)
+  if (dtype == DT_BF16) {
+    if (D == 128) KGC_MERGE(bf16, 128);
+    else KGC_MERGE(bf16, 64);
+  } else {
+    if (D == 128) KGC_MERGE(f16, 128);
+    else KGC_MERGE(f16, 64);
+  }
+#undef KGC_MERGE
+}
+
 int paged_decode_wave_min_pairs() { return decode_wave_enabled() ? decode_wave_min_pairs() : -1; }
 
 KGC_DEBUG_TU(attention_decode)

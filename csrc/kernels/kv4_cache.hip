@@ -1,0 +1,239 @@
+// Writing and reading the 4-bit key / value cache (kv4.h).
+//
+// kv4_write_kernel: q, k, v of a step from the rows of its fused QKV projection, as rope_kv_kernel (rope_cache.hip) for the
+// wider caches: optional per-head RMS norm, NeoX rotation by one position or by one per axis, q stored in T, k and v as
+// e2m1 numbers with their scales.  A thread has the 16-byte chunk pair (c, c + d / 2) of HG heads that lie side by side in the
+// row: the pair is what the rotation needs, four neighbouring lanes hold a block of 32, and cos / sin are loaded once
+// for the heads.
+//
+// k is rotated in 64 bits, where the products are exact and the sum is rounded once, and then to the nearest code: a key
+// next to the border of two codes, which are up to a third apart, then has the code that the mathematics gives it, whatever order of
+// operations a compiler prefers.  Values, and keys that are not rotated, are numbers of T already.
+#include "common.h"
+#include "kv4.h"
+#include "launch.h"
+#include "rope_axes.h"
+
+namespace kgc {
+
+constexpr int KV4_NT = 256;
+
+template <typename T, bool NORM, bool ROPE, bool SL, bool AXES, int HG>
+__global__ __launch_bounds__(KV4_NT) void kv4_write_kernel(
+    const void* __restrict__ qkv, int64_t qkv_stride, int S, int64_t slice_stride, const int64_t* __restrict__ positions,
+    const float* __restrict__ cos_sin, T* __restrict__ q_out, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
+    const int64_t* __restrict__ slot_mapping, const T* __restrict__ qn_w, const T* __restrict__ kn_w, int64_t T_, int nq,
+    int nkv, int d, int bs, float eps, int num_blocks, RopeAxes ax) {
+  const int tph = d >> 4, half = d >> 1;               // threads per head: 4 or 8, whole lane groups
+  const int heads = nq + 2 * nkv, groups = (heads + HG - 1) / HG, per = groups * tph;
+  const int64_t item = (int64_t)blockIdx.x * KV4_NT + threadIdx.x;
+  if (item >= T_ * per) return;                        // whole lane groups
+  const int64_t t = item / per;
+  const int r = (int)(item - t * per), h0 = r / tph * HG, c = r % tph;
+  const int64_t row = t * qkv_stride;
+  int64_t slot = slot_mapping[t];
+  KGC_DCHECK_RANGE(slot, -1, (int64_t)num_blocks * bs, "KV slot");
+  if (slot >= (int64_t)num_blocks * bs) slot = -1;     // beyond the pool: not written
+  const int64_t blk = slot >= 0 ? slot / bs : 0;
+  const int off = slot >= 0 ? (int)(slot - blk * bs) : 0;
+  auto load8 = [&](int col) -> u32x4 {
+    if constexpr (!SL) {
+      return *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(qkv) + row + col);
+    } else {
+      const float* p = reinterpret_cast<const float*>(qkv) + row + col;
+      f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+      for (int z = 1; z < S; ++z) {
+        a += *reinterpret_cast<const f32x4*>(p + z * slice_stride);
+        b += *reinterpret_cast<const f32x4*>(p + z * slice_stride + 4);
+      }
+      Pack8<T> o;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        o.h[q] = from_f<T>(a[q]);
+        o.h[4 + q] = from_f<T>(b[q]);
+      }
+      return o.u;
+    }
+  };
+  Pack8<T> a[HG], b[HG];
+#pragma unroll
+  for (int k = 0; k < HG; ++k) {                       // the last group's missing heads: its last one again
+    const int col = min(h0 + k, heads - 1) * d + c * 8;
+    a[k].u = load8(col);
+    b[k].u = load8(col + half);
+  }
+  float cc[8], sn[8];
+  if constexpr (ROPE) {
+    if (h0 < nq + nkv) {
+      if constexpr (AXES) {
+        axes_cos_sin(ax, positions, (int)t, cos_sin, d, c * 8, cc, sn);
+      } else {
+        int64_t p = positions[t];
+        KGC_DCHECK_RANGE(p, 0, ax.rows, "position");
+        const float* cs = cos_sin + min(max(p, (int64_t)0), (int64_t)ax.rows - 1) * d + c * 8;
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(cs + j), y = *reinterpret_cast<const f32x4*>(cs + half + j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            cc[j + i] = x[i];
+            sn[j + i] = y[i];
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < HG; ++k) {
+    const int head = h0 + k;                           // the same for the head's lanes
+    if (head >= heads) break;
+    float xa[8], xb[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      xa[j] = to_f(a[k].h[j]);
+      xb[j] = to_f(b[k].h[j]);
+    }
+    if (NORM && head < nq + nkv) {
+      const T* w = head < nq ? qn_w : kn_w;
+      Pack8<T> wa, wb;
+      wa.u = *reinterpret_cast<const u32x4*>(w + c * 8);
+      wb.u = *reinterpret_cast<const u32x4*>(w + half + c * 8);
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss += xa[j] * xa[j] + xb[j] * xb[j];
+      for (int o = 1; o < tph; o <<= 1) ss += __shfl_xor(ss, o, 64);
+      const float inv = rsqrtf(ss / (float)d + eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {                    // the norm's own result is one of T
+        xa[j] = to_f(from_f<T>(xa[j] * inv * to_f(wa.h[j])));
+        xb[j] = to_f(from_f<T>(xb[j] * inv * to_f(wb.h[j])));
+      }
+    }
+    if (head < nq) {
+      if constexpr (ROPE) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) neox_rot(xa[j], xb[j], cc[j], sn[j], xa[j], xb[j]);
+      }
+      Pack8<T> oa, ob;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        oa.h[j] = from_f<T>(xa[j]);
+        ob.h[j] = from_f<T>(xb[j]);
+      }
+      T* dst = q_out + (t * nq + head) * d + c * 8;
+      *reinterpret_cast<u32x4*>(dst) = oa.u;
+      *reinterpret_cast<u32x4*>(dst + half) = ob.u;
+      continue;
+    }
+    const bool key = head < nq + nkv;
+    if constexpr (ROPE) {
+      if (key) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const double x = xa[j], y = xb[j], co = cc[j], si = sn[j];
+          xa[j] = round_to_odd(__builtin_fma(x, co, -(y * si)));
+          xb[j] = round_to_odd(__builtin_fma(y, co, x * si));
+        }
+      }
+    }
+    float ma = 0.f, mb = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {                      // e2m1 has no NaN: zero
+      xa[j] = xa[j] == xa[j] ? xa[j] : 0.f;
+      xb[j] = xb[j] == xb[j] ? xb[j] : 0.f;
+      ma = fmaxf(ma, fabsf(xa[j]));
+      mb = fmaxf(mb, fabsf(xb[j]));
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      ma = fmaxf(ma, __shfl_xor(ma, o, 64));
+      mb = fmaxf(mb, __shfl_xor(mb, o, 64));
+    }
+    if (slot < 0) continue;
+    const uint32_t sa = kv4_scale_byte<T>(ma), sb = kv4_scale_byte<T>(mb);
+    uint8_t* page = (key ? k_cache : v_cache) + (blk * nkv + (key ? head - nq : head - nq - nkv)) * kv4_page_bytes(bs, d);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(page + off * (d >> 1));
+    dst[c] = fp4x8(xa, kv4_scale(sa));
+    dst[tph + c] = fp4x8(xb, kv4_scale(sb));
+    if ((c & 3) == 0) {
+      uint8_t* sc = page + bs * (d >> 1) + off * (d >> 5);
+      sc[c >> 2] = (uint8_t)sa;
+      sc[(tph + c) >> 2] = (uint8_t)sb;
+    }
+  }
+}
+
+// Rows of the cache as the values they stand for; slots outside the pool give zeros.  8 elements a thread.
+template <typename T>
+__global__ __launch_bounds__(KV4_NT) void kv4_read_kernel(T* __restrict__ out, const uint8_t* __restrict__ cache,
+                                                          const int64_t* __restrict__ slots, int64_t n, int nkv, int d,
+                                                          int bs, int num_blocks) {
+  const int per = nkv * (d >> 3);
+  const int64_t item = (int64_t)blockIdx.x * KV4_NT + threadIdx.x;
+  if (item >= n * per) return;
+  const int64_t i = item / per;
+  const int r = (int)(item - i * per), h = r / (d >> 3), c = r % (d >> 3);
+  const int64_t slot = slots[i];
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (slot >= 0 && slot < (int64_t)num_blocks * bs) {
+    const int64_t blk = slot / bs;
+    const int off = (int)(slot - blk * bs);
+    const uint8_t* page = cache + (blk * nkv + h) * kv4_page_bytes(bs, d);
+    v = fp4x8_widen<T>(reinterpret_cast<const uint32_t*>(page + off * (d >> 1))[c],
+                       kv4_scale(page[bs * (d >> 1) + off * (d >> 5) + (c >> 2)]));
+  }
+  reinterpret_cast<u32x4*>(out)[item] = v;
+}
+
+template <typename T, bool SL, bool AXES, int HG>
+static void kv4_write_norm(const Kv4Write& w, const RopeAxes& ax, int64_t blocks, hipStream_t s) {
+#define KGC_KV4_WRITE(N, R)                                                                                            \
+  kv4_write_kernel<T, N, R, SL, AXES, HG><<<(unsigned)blocks, KV4_NT, 0, s>>>(                                          \
+      w.qkv, w.qkv_stride, w.S, w.slice_stride, w.positions, w.cos_sin, (T*)w.q_out, (uint8_t*)w.k_cache,               \
+      (uint8_t*)w.v_cache, w.slots, (const T*)w.q_norm_w, (const T*)w.k_norm_w, w.T, w.nq, w.nkv, w.d, w.bs, w.eps,     \
+      w.num_blocks, ax)
+  if constexpr (AXES) {
+    if (w.q_norm_w) KGC_KV4_WRITE(true, true);
+    else KGC_KV4_WRITE(false, true);
+  } else if (w.q_norm_w) {
+    if (w.use_rope) KGC_KV4_WRITE(true, true);
+    else KGC_KV4_WRITE(true, false);
+  } else {
+    if (w.use_rope) KGC_KV4_WRITE(false, true);
+    else KGC_KV4_WRITE(false, false);
+  }
+#undef KGC_KV4_WRITE
+}
+
+template <typename T>
+static void kv4_write_dispatch(const Kv4Write& w, const RopeAxes& ax, hipStream_t s) {
+  auto blocks = [&](int hg) { return (w.T * ((w.nq + 2 * w.nkv + hg - 1) / hg) * (w.d >> 4) + KV4_NT - 1) / KV4_NT; };
+  if (w.S > 0) {
+    if (ax.n) kv4_write_norm<T, true, true, 1>(w, ax, blocks(1), s);
+    else kv4_write_norm<T, true, false, 1>(w, ax, blocks(1), s);
+  } else if (ax.n) {
+    kv4_write_norm<T, false, true, 4>(w, ax, blocks(4), s);
+  } else {
+    kv4_write_norm<T, false, false, 4>(w, ax, blocks(4), s);
+  }
+}
+
+void launch_kv4_write(int dtype, const Kv4Write& w, const RopeAxes& ax, hipStream_t s) {
+  if (w.T == 0) return;
+  if (dtype == DT_BF16) kv4_write_dispatch<bf16>(w, ax, s);
+  else kv4_write_dispatch<f16>(w, ax, s);
+}
+
+void launch_kv4_read(int dtype, void* out, const void* cache, const int64_t* slots, int64_t n, int nkv, int d, int bs,
+                     int num_blocks, hipStream_t s) {
+  if (n == 0) return;
+  const unsigned blocks = (unsigned)((n * nkv * (d >> 3) + KV4_NT - 1) / KV4_NT);
+  if (dtype == DT_BF16)
+    kv4_read_kernel<<<blocks, KV4_NT, 0, s>>>((bf16*)out, (const uint8_t*)cache, slots, n, nkv, d, bs, num_blocks);
+  else
+    kv4_read_kernel<<<blocks, KV4_NT, 0, s>>>((f16*)out, (const uint8_t*)cache, slots, n, nkv, d, bs, num_blocks);
+}
+
+KGC_DEBUG_TU(kv4_cache)
+
+}  // namespace kgc

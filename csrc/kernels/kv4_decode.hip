@@ -1,0 +1,227 @@
+// Paged-attention decode over the 4-bit cache (kv4.h): one query row per sequence.
+//
+// One wave per (sequence, kv head, z-slice), as paged_decode_wave_kernel (attention_decode.hip) and with its slices
+// (decode_slices.h) and its merge.  A chunk is 32 tokens, two groups of 16; a page holds 16 or more, so that a group lies in
+// one.  Lane (token r16 of a group, quarter qd of the head) loads its quarter row with one load of D / 8 bytes, and the
+// scale with it; next chunk's loads are on their way while one computes.
+//   S^T[token][head] = K Q^T: the quarter row, widened, is the operand of D / 32 MFMAs as it is -- their contraction takes the
+//                      head's elements in the order (quarter, 8 of it, next 8 ..), and so does q's operand
+//   O^T[d][head]    += V^T P^T: the widened rows go through LDS, where the transposing reads make columns of them; the
+//                      contraction's order of tokens is that of S^T's accumulator, so that P needs no exchange
+#include "common.h"
+#include "decode_slices.h"
+#include "kv4.h"
+#include "launch.h"
+
+namespace kgc {
+
+__device__ __forceinline__ float kv4_max_rows(float x) {     // over the four lanes that share lane & 15
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(64, 2) void kv4_decode_kernel(
+    T* __restrict__ out, const T* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+    const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ ctx_lens, float* __restrict__ max_logits,
+    float* __restrict__ exp_sums, float* __restrict__ tmp_out, int nq, int nkv, int bs_log2, float scale_log2,
+    int num_blocks, DecodeLeast least) {
+  typedef typename Vec8<T>::type V8;
+  constexpr int KS = D / 32, DT = D / 16, VS = D + 16;       // VS: the 4 rows x 32 bytes of a transposing read on 32 banks
+  __shared__ __attribute__((aligned(16))) T lds_v[32 * VS];
+  const int b = blockIdx.x, h = blockIdx.y, z = blockIdx.z, Z = gridDim.z;
+  const int lane = threadIdx.x, r16 = lane & 15, qd = lane >> 4;
+  const int G = nq / nkv;
+  int ctx_in = ctx_lens[b];
+  KGC_DCHECK_RANGE(ctx_in, 0, (bt_stride << bs_log2) + 1, "decode ctx_len");
+  const int ctx = min(ctx_in, bt_stride << bs_log2);         // a bad length gives wrong output, never a fault
+  const int* bt = block_tables + (int64_t)b * bt_stride;
+  const int bs = 1 << bs_log2, bsm = bs - 1;
+  const int64_t page_bytes = kv4_page_bytes(bs, D);
+
+  const int nchunk = (max(ctx, 0) + 31) >> 5;
+  const int min_per = decode_min_chunks(least, nchunk);
+  const int per = decode_slice_chunks(nchunk, Z, min_per);
+  const int nused = decode_used_slices(nchunk, Z, min_per);
+  const int c0 = min(nchunk, z * per), c1 = min(nchunk, c0 + per);
+  const int end = min(ctx, c1 << 5);                         // this wave's tokens: [32 c0, end)
+
+  struct Frag {
+    uint32_t k[2][KS], v[2][KS];
+    uint8_t ks[2], vs[2];
+  };
+  auto load = [&](uint32_t (&w)[KS], const uint8_t* p) {
+    if constexpr (KS == 4) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+      w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+    } else {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+      w[0] = x.x; w[1] = x.y;
+    }
+  };
+  auto issue = [&](Frag& f, int ci) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      // tokens behind the slice's last one are that one again: their scores are masked
+      const int t0 = min((ci << 5) + 16 * g, end - 1), tok = min((ci << 5) + 16 * g + r16, end - 1);
+      const int64_t page = ((int64_t)kgc_bt(bt, t0 >> bs_log2, bt_stride, num_blocks) * nkv + h) * page_bytes;
+      const int row = tok & bsm;
+      const int at = row * (D / 2) + qd * (D / 8), sc = bs * (D / 2) + row * (D / 32) + (qd * D / 4) / 32;
+      load(f.k[g], kc + page + at);
+      load(f.v[g], vc + page + at);
+      f.ks[g] = kc[page + sc];
+      f.vs[g] = vc[page + sc];
+    }
+  };
+
+  float m_run = -INFINITY, l_run = 0.f;
+  f32x4 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Frag fa, fb;
+  if (c0 < c1) {
+    issue(fa, c0);
+    issue(fb, min(c0 + 1, c1 - 1));
+  }
+  V8 qf[KS];
+  {
+    const bool valid = r16 < G;
+    const T* qrow = q + ((int64_t)b * nq + h * G + (valid ? r16 : 0)) * D + qd * (D / 4);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      Pack8<T> t;
+      t.u = *reinterpret_cast<const u32x4*>(qrow + 8 * s);
+      if (!valid) t.u = u32x4{0, 0, 0, 0};
+      qf[s] = t.v;
+    }
+  }
+  auto compute = [&](const Frag& f, int ci) {
+    const int base = ci << 5;
+    f32x4 sc[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const float size = kv4_scale(f.ks[g]);
+      sc[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        Pack8<T> kf;
+        kf.u = fp4x8_widen<T>(f.k[g][s], size);
+        sc[g] = mfma16x16x32(kf.v, qf[s], sc[g]);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const float size = kv4_scale(f.vs[g]);
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        *reinterpret_cast<u32x4*>(lds_v + (16 * g + r16) * VS + qd * (D / 4) + 8 * s) = fp4x8_widen<T>(f.v[g][s], size);
+    }
+    asm volatile("" ::: "memory");          // one wave: its LDS operations are in order
+    float m = m_run;
+    if (base + 32 <= end) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sc[g][i] *= scale_log2;
+          m = fmaxf(m, sc[g][i]);
+        }
+    } else {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sc[g][i] = base + 16 * g + 4 * qd + i < end ? sc[g][i] * scale_log2 : -INFINITY;
+          m = fmaxf(m, sc[g][i]);
+        }
+    }
+    m = kv4_max_rows(m);
+    // a row none of whose scores is above -inf (q or k too large): no difference of infinities
+    const float ref = m == -INFINITY ? 0.f : m;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - ref);
+    m_run = m;
+    l_run *= alpha;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] *= alpha;
+    // probabilities are at most 1 and rounded to T for the product, as the keys' and values' type has it; their sum is not
+    Pack8<T> pf;
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = __builtin_amdgcn_exp2f(sc[g][i] - ref);
+        l_run += p;
+        pf.h[4 * g + i] = from_f<T>(p);
+      }
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      const T* src = lds_v + (4 * qd + (r16 >> 2)) * VS + 16 * t + 4 * (r16 & 3);
+      const u32x2 lo = ld_tr4(src), hi = ld_tr4(src + 16 * VS);
+      Pack8<T> vf;
+      vf.u = u32x4{lo.x, lo.y, hi.x, hi.y};
+      o[t] = mfma16x16x32(vf.v, pf.v, o[t]);
+    }
+    asm volatile("" ::: "memory");
+  };
+  // straight-line, two chunks deep: behind the last one a chunk is computed masked (p = 0, alpha = 1)
+  for (int ci = c0; ci < c1; ci += 2) {
+    compute(fa, ci);
+    issue(fa, min(ci + 2, c1 - 1));
+    compute(fb, ci + 1);
+    issue(fb, min(ci + 3, c1 - 1));
+  }
+
+  l_run += __shfl_xor(l_run, 16, 64);
+  l_run += __shfl_xor(l_run, 32, 64);
+  const int64_t row = (int64_t)b * nq + h * G + r16;
+  if (Z == 1 || nused == 1) {               // the whole context: the merge skips such a row
+    if (z > 0 || r16 >= G) return;
+    const float inv = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f;
+    T* orow = out + row * D + 4 * qd;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      Pack4<T> pk;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pk.h[i] = from_f<T>(o[t][i] * inv);
+      *reinterpret_cast<u32x2*>(orow + 16 * t) = pk.u;
+    }
+    return;
+  }
+  if (z >= nused || r16 >= G) return;
+  const int64_t prow = row * Z + z;
+  float* dst = tmp_out + prow * D + 4 * qd;
+#pragma unroll
+  for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(dst + 16 * t) = o[t];
+  if (qd == 0) {
+    max_logits[prow] = m_run;
+    exp_sums[prow] = l_run;
+  }
+}
+
+template <typename T>
+static void kv4_decode_dispatch(const Kv4Decode& a, DecodeLeast least, float sl2, hipStream_t s) {
+#define KGC_KV4_DEC(DD)                                                                                                \
+  kv4_decode_kernel<T, DD><<<dim3(a.B, a.nkv, a.Z), 64, 0, s>>>(                                                         \
+      (T*)a.out, (const T*)a.q, (const uint8_t*)a.k_cache, (const uint8_t*)a.v_cache, a.block_tables, a.bt_stride,      \
+      a.ctx_lens, a.max_logits, a.exp_sums, a.tmp_out, a.nq, a.nkv, a.bs_log2, sl2, a.num_blocks, least)
+  if (a.D == 128) KGC_KV4_DEC(128);
+  else KGC_KV4_DEC(64);
+#undef KGC_KV4_DEC
+}
+
+void launch_kv4_decode(int dtype, const Kv4Decode& a, float scale, hipStream_t s) {
+  if (a.B == 0) return;
+  const DecodeLeast least{-1, 2, 2};
+  const float sl2 = scale * 1.4426950408889634f;
+  if (dtype == DT_BF16) kv4_decode_dispatch<bf16>(a, least, sl2, s);
+  else kv4_decode_dispatch<f16>(a, least, sl2, s);
+  if (a.Z > 1)
+    launch_paged_decode_merge(dtype, a.out, a.max_logits, a.exp_sums, a.tmp_out, a.ctx_lens, a.B, a.nq, a.D, a.Z,
+                              a.bt_stride << a.bs_log2, least, s);
+}
+
+KGC_DEBUG_TU(kv4_decode)
+
+}  // namespace kgc

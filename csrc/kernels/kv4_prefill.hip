@@ -1,0 +1,221 @@
+// Causal attention of a step's prompt rows over the 4-bit cache (kv4.h): fresh prompts and chunks that continue one.
+//
+// A workgroup of 4 waves has 32 query rows of each of GH heads of one kv head (GH = 1, 2, 4; GH * 32 of the 128-row work item's
+// rows with 4 / GH of its blocks).  Keys and values advance in tiles of 64 tokens: a thread loads a quarter row of K and
+// of V (D / 8 bytes each) while the tile before it computes, widens them and writes them to LDS as T, in two buffers, one
+// barrier per tile.  So a tile is widened once for 128 rows of queries, and a wave widens D / 32 * 4 instructions' worth of it beside
+// its own 4 * D / 8 MFMAs.
+//
+// v_mfma_f32_32x32x16: S^T = K Q^T and O^T = V^T P^T, so that a query is a lane's column in every accumulator: its maximum
+// and sum are the lane's own (and its partner's, lane ^ 32), and S^T's accumulator, packed, is the B operand of the second product.
+// V's rows become columns by the transposing LDS read.
+#include "common.h"
+#include "kv4.h"
+#include "launch.h"
+
+namespace kgc {
+
+constexpr int KV4_BM = 128, KV4_BN = 64;
+
+__device__ __forceinline__ float kv4_max_pair(float x) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+template <typename T, int D, int GH>
+__global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
+    const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+    const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ qsl, const int* __restrict__ seq_lens,
+    const int* __restrict__ work_seq, const int* __restrict__ work_mblk, int nq, int nkv, int bs_log2, float scale_log2,
+    int num_blocks) {
+  typedef typename Vec8<T>::type V8;
+  constexpr int QB = KV4_BM / GH;                    // query rows of a workgroup
+  constexpr int KS = D / 16, DT = D / 32, W = D / 32; // W: words of a thread's quarter row
+  constexpr int KST = D + 8, VST = D + 16;           // rows of the LDS tiles: a wave's 16-byte and transposing reads spread over the banks
+  __shared__ __attribute__((aligned(16))) T lds_k[2][KV4_BN * KST], lds_v[2][KV4_BN * VST];
+  const int seq = work_seq[blockIdx.x], mb = work_mblk[blockIdx.x];
+  const int G = nq / nkv, h = blockIdx.y / (G / GH), head0 = h * G + blockIdx.y % (G / GH) * GH;
+  const int q0 = qsl[seq], qlen = qsl[seq + 1] - q0;
+  int L_in = seq_lens[seq];
+  KGC_DCHECK_RANGE(L_in, 0, (bt_stride << bs_log2) + 1, "prefill seq_len");
+  const int L = min(L_in, bt_stride << bs_log2), ctx0 = L - qlen;
+  const int qbase = mb * KV4_BM + blockIdx.z * QB;
+  if (qlen <= 0 || ctx0 < 0 || qbase >= qlen) return;  // the whole workgroup
+  const int* bt = block_tables + (int64_t)seq * bt_stride;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, hi = lane >> 5;
+  const int bs = 1 << bs_log2, bsm = bs - 1;
+  const int64_t page_bytes = kv4_page_bytes(bs, D);
+  const int wrow = qbase + wave / GH * 32, head = head0 + wave % GH;
+  const int tiles = (ctx0 + min(qbase + QB, qlen) - 1) / KV4_BN + 1;
+  // no row of this wave sees further (it may have none)
+  const int wave_tiles = wrow < qlen ? (ctx0 + min(wrow + 32, qlen) - 1) / KV4_BN + 1 : 0;
+
+  const int tok = tid >> 2, part = tid & 3;            // of the tile's rows
+  uint32_t kw[W], vw[W];
+  uint8_t ks, vs;
+  auto page_of = [&](int kt) { return kgc_bt(bt, min(kt * KV4_BN + tok, L - 1) >> bs_log2, bt_stride, num_blocks); };
+  auto load = [&](int kt, int pg) {                    // tokens behind the last one are that one again, and masked
+    const int64_t page = ((int64_t)pg * nkv + h) * page_bytes;
+    const int row = min(kt * KV4_BN + tok, L - 1) & bsm;
+    const int at = row * (D / 2) + part * (D / 8), sc = bs * (D / 2) + row * (D / 32) + (part * D / 4) / 32;
+    if constexpr (W == 4) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(kc + page + at), y = *reinterpret_cast<const u32x4*>(vc + page + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { kw[i] = x[i]; vw[i] = y[i]; }
+    } else {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(kc + page + at), y = *reinterpret_cast<const u32x2*>(vc + page + at);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) { kw[i] = x[i]; vw[i] = y[i]; }
+    }
+    ks = kc[page + sc];
+    vs = vc[page + sc];
+  };
+  auto store = [&](int buf) {
+    const float a = kv4_scale(ks), b = kv4_scale(vs);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      *reinterpret_cast<u32x4*>(&lds_k[buf][tok * KST + part * (D / 4) + 8 * i]) = fp4x8_widen<T>(kw[i], a);
+      *reinterpret_cast<u32x4*>(&lds_v[buf][tok * VST + part * (D / 4) + 8 * i]) = fp4x8_widen<T>(vw[i], b);
+    }
+  };
+
+  int pg = page_of(0);
+  load(0, pg);
+  pg = page_of(min(1, tiles - 1));
+  // q: lane (row col, hi) has elements 16 s + 8 hi .. + 7; rows behind the prompt's last one are that one again, not stored
+  const int qi = min(wrow + col, qlen - 1), qpos = ctx0 + qi;
+  V8 qf[KS];
+  {
+    const T* qrow = q + ((int64_t)(q0 + qi) * nq + head) * D + 8 * hi;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      Pack8<T> t;
+      t.u = *reinterpret_cast<const u32x4*>(qrow + 16 * s);
+      qf[s] = t.v;
+    }
+  }
+  store(0);
+  __syncthreads();
+  f32x16 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  for (int kt = 0; kt < tiles; ++kt) {
+    const int buf = kt & 1;
+    if (kt + 1 < tiles) {
+      load(kt + 1, pg);
+      pg = page_of(min(kt + 2, tiles - 1));
+    }
+    if (kt < wave_tiles) {
+      const T* K = lds_k[buf];
+      const T* V = lds_v[buf];
+      f32x16 s[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[g][i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          Pack8<T> kf;
+          kf.u = *reinterpret_cast<const u32x4*>(K + (32 * g + col) * KST + 16 * j + 8 * hi);
+          s[g] = mfma32x32x16(kf.v, qf[j], s[g]);
+        }
+      }
+      const int key0 = kt * KV4_BN + 4 * hi;           // element i of half g: key0 + 32 g + 8 (i / 4) + i % 4
+      if (kt * KV4_BN + KV4_BN - 1 > ctx0 + wrow) {    // some row of the wave does not see all of the tile
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (key0 + 32 * g + 8 * (i >> 2) + (i & 3) > qpos) s[g][i] = -INFINITY;
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[g][i]);
+      top = kv4_max_pair(top) * scale_log2;
+      // the maximum moves only where it grows by more than 8: probabilities are then at most 2^8, and O is seldom rescaled
+      if (__any(top > m + 8.f)) {
+        const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] *= f;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      V8 pf[4];
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          Pack8<T> p;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g][8 * j + i], scale_log2, -ref));
+            l += e;
+            p.h[i] = from_f<T>(e);                     // at most 2^8; the sum keeps 32 bits
+          }
+          pf[2 * g + j] = p.v;
+        }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          const T* src = V + (16 * j + 4 * hi + ((lane & 15) >> 2)) * VST + 32 * t + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+          const u32x2 a = ld_tr4(src), b = ld_tr4(src + 8 * VST);
+          Pack8<T> vf;
+          vf.u = u32x4{a.x, a.y, b.x, b.y};
+          o[t] = mfma32x32x16(vf.v, pf[j], o[t]);
+        }
+    }
+    if (kt + 1 < tiles) {
+      store(buf ^ 1);
+      __syncthreads();
+    }
+  }
+  if (wrow + col >= qlen) return;
+  l += __shfl_xor(l, 32, 64);
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  T* orow = out + ((int64_t)(q0 + qi) * nq + head) * D + 4 * hi;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      Pack4<T> pk;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pk.h[i] = from_f<T>(o[t][4 * j + i] * inv);
+      *reinterpret_cast<u32x2*>(orow + 32 * t + 8 * j) = pk.u;
+    }
+}
+
+template <typename T, int D>
+static void kv4_prefill_dispatch(const Kv4Prefill& a, float sl2, hipStream_t s) {
+  const int G = a.nq / a.nkv;
+#define KGC_KV4_PF(GH)                                                                                                \
+  kv4_prefill_kernel<T, D, GH><<<dim3(a.n_work, a.nkv * (G / GH), GH), 256, 0, s>>>(                                     \
+      (const T*)a.q, (T*)a.out, (const uint8_t*)a.k_cache, (const uint8_t*)a.v_cache, a.block_tables, a.bt_stride,      \
+      a.query_start_loc, a.seq_lens, a.work_seq, a.work_mblk, a.nq, a.nkv, a.bs_log2, sl2, a.num_blocks)
+  if (G % 4 == 0) KGC_KV4_PF(4);
+  else if (G % 2 == 0) KGC_KV4_PF(2);
+  else KGC_KV4_PF(1);
+#undef KGC_KV4_PF
+}
+
+void launch_kv4_prefill(int dtype, const Kv4Prefill& a, float scale, hipStream_t s) {
+  if (a.n_work == 0) return;
+  const float sl2 = scale * 1.4426950408889634f;
+  if (dtype == DT_BF16) {
+    if (a.D == 128) kv4_prefill_dispatch<bf16, 128>(a, sl2, s);
+    else kv4_prefill_dispatch<bf16, 64>(a, sl2, s);
+  } else {
+    if (a.D == 128) kv4_prefill_dispatch<f16, 128>(a, sl2, s);
+    else kv4_prefill_dispatch<f16, 64>(a, sl2, s);
+  }
+}
+
+KGC_DEBUG_TU(kv4_prefill)
+
+}  // namespace kgc

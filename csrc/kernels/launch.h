@@ -14,13 +14,14 @@ void launch_layer_norm(int dtype, void* out, const void* x, const void* w, const
                        int rows, int H, float eps, hipStream_t s);
 void launch_silu_mul(int dtype, void* out, int64_t os, const void* x, int64_t xs, int64_t rows,
                      int I, hipStream_t s);
+struct RopeAxes;             // rope_axes.h; n = 0: one position per token
 // S > 0: qkv is S fp32 split-K slices [S, T, qkv_stride] (slice_stride apart), summed here
 void launch_rope_kv_write(int dtype, const void* qkv, int64_t qkv_stride, int S,
                           int64_t slice_stride, const int64_t* positions, const float* cos_sin, void* q_out,
                           void* k_cache, void* v_cache, const int64_t* slot_mapping,
                           const void* q_norm_w, const void* k_norm_w, int T, int nq, int nkv,
                           int d, int bs, float eps, bool use_rope, bool kv_fp8, float k_scale,
-                          float v_scale, int num_blocks, hipStream_t s);
+                          float v_scale, int num_blocks, const RopeAxes& ax, hipStream_t s);
 // Z > 1: the partials hold B * nq * Z rows (row (seq, q-head) * Z + z), merged by a
 // reduce launch
 void launch_paged_decode(int dtype, void* out, const void* q, const void* k_cache,
@@ -71,11 +72,53 @@ void launch_prefill_attention(int dtype, const void* q, void* out, const void* k
                               int nkv, int D, int bs_log2, float scale, bool kv_fp8,
                               float k_scale, float v_scale, int num_blocks, int64_t q_stride,
                               const float* cos_sin, int cs_rows, hipStream_t s);
+// The merge of K1w's partials by itself, for a decode kernel of its own that cuts contexts the same way (``least``:
+// decode_slices.h) and writes the rows of single slices itself.
+struct DecodeLeast;
+void launch_paged_decode_merge(int dtype, void* out, const float* max_logits, const float* exp_sums, const float* tmp_out,
+                               const int* ctx_lens, int B, int nq, int D, int Z, int ctx_cap, const DecodeLeast& least,
+                               hipStream_t s);
+// ---- the cache in 4 bits (kv4.h)
+struct Kv4Write {
+  const void* qkv;           // T [T, qkv_stride], or S > 0 fp32 slices [S, T, qkv_stride], slice_stride apart
+  int64_t qkv_stride, slice_stride;
+  int S;
+  const int64_t* positions;
+  const float* cos_sin;
+  void *q_out, *k_cache, *v_cache;
+  const int64_t* slots;
+  const void *q_norm_w, *k_norm_w;           // nullptr: no q / k RMS norm
+  int64_t T;
+  int nq, nkv, d, bs, num_blocks;
+  float eps;
+  bool use_rope;
+};
+void launch_kv4_write(int dtype, const Kv4Write& w, const RopeAxes& ax, hipStream_t s);
+void launch_kv4_read(int dtype, void* out, const void* cache, const int64_t* slots, int64_t n, int nkv, int d, int bs,
+                     int num_blocks, hipStream_t s);
+struct Kv4Decode {
+  const void *q, *k_cache, *v_cache;
+  void* out;
+  const int *block_tables, *ctx_lens;
+  float *max_logits, *exp_sums, *tmp_out;
+  int bt_stride, B, nq, nkv, D, bs_log2, Z, num_blocks;
+};
+void launch_kv4_decode(int dtype, const Kv4Decode& a, float scale, hipStream_t s);
+struct Kv4Prefill {
+  const void *q, *k_cache, *v_cache;
+  void* out;
+  const int *block_tables, *query_start_loc, *seq_lens, *work_seq, *work_mblk;
+  int bt_stride, n_work, nq, nkv, D, bs_log2, num_blocks;
+};
+void launch_kv4_prefill(int dtype, const Kv4Prefill& a, float scale, hipStream_t s);
 // debug builds: sticky bounds-check error words of the K1 / K2 / K3 translation units
 // (read and cleared; always 0 in release builds)
 uint32_t dbg_err_attention_decode();
 uint32_t dbg_err_attention_prefill();
 uint32_t dbg_err_rope_cache();
+uint32_t dbg_err_kv4_decode();
+uint32_t dbg_err_kv4_prefill();
+uint32_t dbg_err_kv4_cache();
 int prefill_block_m();
 int sample_splits(int B);   // vocabulary splits per row; partial holds B * splits words
 void launch_sample(int dtype, int64_t* out, uint64_t* partial, const void* logits,

@@ -13,6 +13,7 @@
 // quantised is the T-rounded one, exactly what a T cache would store.
 #include "common.h"
 #include "launch.h"
+#include "rope_axes.h"
 #include <climits>
 #include <cstdlib>
 #include <type_traits>
@@ -59,14 +60,15 @@ __device__ __forceinline__ u32x2 fp8_8(const Pack8<T>& v, float inv) {
 
 // KVO: k / v only (q_out unused): the prefill attention kernel rotates q itself as it
 // loads it from the QKV row, so a prefill-only step never writes or re-reads q
-template <typename T, bool NORM, bool ROPE, bool KV8, bool SL, bool KVO>
+// AXES: a position per axis and token (rope_axes.h), q / k / v
+template <typename T, bool NORM, bool ROPE, bool KV8, bool SL, bool KVO, bool AXES>
 __global__ __launch_bounds__(ROPE_NT) void rope_kv_kernel(
     const void* __restrict__ qkv, int64_t qkv_stride, int S, int64_t slice_stride,
     const int64_t* __restrict__ positions,
     const float* __restrict__ cos_sin, T* __restrict__ q_out, void* __restrict__ k_cache,
     void* __restrict__ v_cache, const int64_t* __restrict__ slot_mapping,
     const T* __restrict__ qn_w, const T* __restrict__ kn_w, int nq, int nkv, int d, int bs,
-    float eps, float k_inv, float v_inv, int num_blocks) {
+    float eps, float k_inv, float v_inv, int num_blocks, RopeAxes ax) {
   // item space of one token: [q/k rotation items, padded to a wave] [v scatter items];
   // gridDim.y workgroups of ROPE_NT items share a token (fills the CUs at decode).
   // A q/k item is one chunk pair (c, c + d/2) of a group of ROPE_HG heads: the position's
@@ -100,7 +102,9 @@ __global__ __launch_bounds__(ROPE_NT) void rope_kv_kernel(
       b[k].u = qkv8<T, SL>(qkv, row + head * d, half + c * 8, S, slice_stride);
     }
     float cc[8], sn[8];
-    if (ROPE) {
+    if constexpr (AXES) {
+      axes_cos_sin(ax, positions, t, cos_sin, d, c * 8, cc, sn);
+    } else if (ROPE) {
       const float* cs = cos_sin + positions[t] * d;
       const float4 c0 = *reinterpret_cast<const float4*>(cs + c * 8);
       const float4 c1 = *reinterpret_cast<const float4*>(cs + c * 8 + 4);
@@ -374,18 +378,24 @@ static void rope_dispatch(const void* qkv, int64_t qkv_stride, int S, int64_t ss
                           const float* cs, void* q_out, void* kc, void* vc,
                           const int64_t* slots, const void* qn, const void* kn, int T_,
                           int nq, int nkv, int d, int bs, float eps, bool rope, float k_inv,
-                          float v_inv, int num_blocks, hipStream_t s) {
+                          float v_inv, int num_blocks, const RopeAxes& ax, hipStream_t s) {
   if (T_ == 0) return;
   const bool kvo = q_out == nullptr;
   constexpr int HG = rope_hg<SL>();
   const int n_items = (((((kvo ? 0 : nq) + nkv) + HG - 1) / HG * (d >> 4) + 63) & ~63) +
                       nkv * (d >> 3);
   const dim3 grid(T_, (n_items + ROPE_NT - 1) / ROPE_NT);
-#define KGC_ROPE_LAUNCH(N, R, O)                                                            \
-  rope_kv_kernel<T, N, R, KV8, SL, O><<<grid, ROPE_NT, 0, s>>>(                             \
+#define KGC_ROPE_LAUNCH_AXES(N, R, O, A)                                                    \
+  rope_kv_kernel<T, N, R, KV8, SL, O, A><<<grid, ROPE_NT, 0, s>>>(                          \
       qkv, qkv_stride, S, ss, pos, cs, (T*)q_out, kc, vc, slots, (const T*)qn,               \
-      (const T*)kn, nq, nkv, d, bs, eps, k_inv, v_inv, num_blocks)
+      (const T*)kn, nq, nkv, d, bs, eps, k_inv, v_inv, num_blocks, ax)
+#define KGC_ROPE_LAUNCH(N, R, O) KGC_ROPE_LAUNCH_AXES(N, R, O, false)
   const bool norm = qn != nullptr;
+  if (ax.n) {                   // (the host: rotated, q asked for)
+    if (norm) KGC_ROPE_LAUNCH_AXES(true, true, false, true);
+    else KGC_ROPE_LAUNCH_AXES(false, true, false, true);
+    return;
+  }
   if constexpr (!SL) {
     const int64_t slots_end = (int64_t)num_blocks * bs;
     if (kvo && rope && !norm && rope_kvg() && (d & 15) == 0 && (bs & 7) == 0 && slots_end < INT_MAX) {
@@ -406,6 +416,7 @@ static void rope_dispatch(const void* qkv, int64_t qkv_stride, int S, int64_t ss
   else if (rope) KGC_ROPE_LAUNCH(false, true, false);
   else KGC_ROPE_LAUNCH(false, false, false);
 #undef KGC_ROPE_LAUNCH
+#undef KGC_ROPE_LAUNCH_AXES
 }
 
 template <typename T, bool KV8>
@@ -413,13 +424,13 @@ static void rope_dispatch_sl(const void* qkv, int64_t qkv_stride, int S, int64_t
                              const int64_t* pos, const float* cs, void* q_out, void* kc, void* vc,
                              const int64_t* slots, const void* qn, const void* kn, int T_,
                              int nq, int nkv, int d, int bs, float eps, bool rope, float k_inv,
-                             float v_inv, int num_blocks, hipStream_t s) {
+                             float v_inv, int num_blocks, const RopeAxes& ax, hipStream_t s) {
   if (S > 0)
     rope_dispatch<T, KV8, true>(qkv, qkv_stride, S, ss, pos, cs, q_out, kc, vc, slots, qn, kn,
-                                T_, nq, nkv, d, bs, eps, rope, k_inv, v_inv, num_blocks, s);
+                                T_, nq, nkv, d, bs, eps, rope, k_inv, v_inv, num_blocks, ax, s);
   else
     rope_dispatch<T, KV8, false>(qkv, qkv_stride, 0, 0, pos, cs, q_out, kc, vc, slots, qn, kn,
-                                 T_, nq, nkv, d, bs, eps, rope, k_inv, v_inv, num_blocks, s);
+                                 T_, nq, nkv, d, bs, eps, rope, k_inv, v_inv, num_blocks, ax, s);
 }
 
 void launch_rope_kv_write(int dtype, const void* qkv, int64_t qkv_stride, int S,
@@ -428,26 +439,26 @@ void launch_rope_kv_write(int dtype, const void* qkv, int64_t qkv_stride, int S,
                           const int64_t* slot_mapping, const void* q_norm_w,
                           const void* k_norm_w, int T, int nq, int nkv, int d, int bs,
                           float eps, bool use_rope, bool kv_fp8, float k_scale, float v_scale,
-                          int num_blocks, hipStream_t s) {
+                          int num_blocks, const RopeAxes& ax, hipStream_t s) {
   const float ki = 1.f / k_scale, vi = 1.f / v_scale;
   if (dtype == DT_BF16) {
     if (kv_fp8)
       rope_dispatch_sl<bf16, true>(qkv, qkv_stride, S, slice_stride, positions, cos_sin, q_out,
                                    k_cache, v_cache, slot_mapping, q_norm_w, k_norm_w, T, nq,
-                                   nkv, d, bs, eps, use_rope, ki, vi, num_blocks, s);
+                                   nkv, d, bs, eps, use_rope, ki, vi, num_blocks, ax, s);
     else
       rope_dispatch_sl<bf16, false>(qkv, qkv_stride, S, slice_stride, positions, cos_sin, q_out,
                                     k_cache, v_cache, slot_mapping, q_norm_w, k_norm_w, T, nq,
-                                    nkv, d, bs, eps, use_rope, ki, vi, num_blocks, s);
+                                    nkv, d, bs, eps, use_rope, ki, vi, num_blocks, ax, s);
   } else {
     if (kv_fp8)
       rope_dispatch_sl<f16, true>(qkv, qkv_stride, S, slice_stride, positions, cos_sin, q_out,
                                   k_cache, v_cache, slot_mapping, q_norm_w, k_norm_w, T, nq,
-                                  nkv, d, bs, eps, use_rope, ki, vi, num_blocks, s);
+                                  nkv, d, bs, eps, use_rope, ki, vi, num_blocks, ax, s);
     else
       rope_dispatch_sl<f16, false>(qkv, qkv_stride, S, slice_stride, positions, cos_sin, q_out,
                                    k_cache, v_cache, slot_mapping, q_norm_w, k_norm_w, T, nq,
-                                   nkv, d, bs, eps, use_rope, ki, vi, num_blocks, s);
+                                   nkv, d, bs, eps, use_rope, ki, vi, num_blocks, ax, s);
   }
 }
 

@@ -20,7 +20,7 @@ _DTYPES = {"auto": None, "bfloat16": torch.bfloat16, "bf16": torch.bfloat16,
            "float32": torch.float32, "float": torch.float32}
 
 
-KV_CACHE_DTYPES = ("auto", "bfloat16", "bf16", "float16", "fp16", "fp8", "fp8_e4m3")
+KV_CACHE_DTYPES = ("auto", "bfloat16", "bf16", "float16", "fp16", "fp8", "fp8_e4m3", "fp4", "fp4_e2m1")
 
 
 @dataclasses.dataclass
@@ -73,7 +73,10 @@ class EngineConfig:
         return model_default if d is None else d
 
     def kv_torch_dtype(self, act: torch.dtype) -> torch.dtype:
-        """Cache element type: fp8 e4m3 for --kv-cache-dtype fp8, else the activations'."""
+        """Cache element type: fp8 e4m3 for --kv-cache-dtype fp8, bytes of two e2m1 numbers each
+        for fp4, else the activations'."""
+        if self.kv_cache_dtype in ("fp4", "fp4_e2m1"):
+            return torch.uint8
         if self.kv_cache_dtype in ("fp8", "fp8_e4m3"):
             return torch.float8_e4m3fn
         return act
@@ -137,7 +140,8 @@ def add_engine_args(p: argparse.ArgumentParser) -> argparse.ArgumentParser:
     a("--disable-custom-all-reduce", action="store_true")
     a("--trust-remote-code", action="store_true")
     a("--kv-cache-dtype", type=str, default="auto",
-      help="auto (activation dtype) or fp8 / fp8_e4m3 (half the KV bytes)")
+      help="auto (activation dtype), fp8 / fp8_e4m3 (half the KV bytes) or fp4 / fp4_e2m1 (4.25 bits "
+           "an element; Llama-style models with heads of 64 or 128)")
     a("--seed", type=int, default=0)
     a("--random-init", action="store_true", help="random weights (offline benchmarking)")
     a("--load-format", type=str, default="auto", help="'dummy' == --random-init")

@@ -80,7 +80,7 @@ class LLMEngine:
             raise ValueError(
                 f"KV cache holds {max(cap, 0)} tokens ({nb} blocks of {cfg.block_size}), less than "
                 f"max_model_len={self.max_model_len}: raise --gpu-memory-utilization, lower "
-                f"--max-model-len, use --kv-cache-dtype fp8, or add tensor parallelism")
+                f"--max-model-len, use --kv-cache-dtype fp8 or fp4, or add tensor parallelism")
         executor.init_cache(nb)
         self.graph_s = executor.capture()
         self.num_blocks = nb

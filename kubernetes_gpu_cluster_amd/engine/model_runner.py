@@ -108,8 +108,16 @@ class ModelRunner:
                  kv_dtype: Optional[torch.dtype] = None, kv_scales: tuple = (1.0, 1.0)):
         self.model, self.mcfg, self.dtype, self.device = model, mcfg, dtype, device
         # KV cache element type: the activation dtype, or fp8 e4m3 (--kv-cache-dtype fp8:
-        # half the bytes per cached token, twice the tokens per GB)
+        # half the bytes per cached token, twice the tokens per GB), or bytes of two e2m1
+        # numbers (fp4: 17/64 of 16-bit bytes, blocks of 32 with scales in the page)
         self.kv_dtype = kv_dtype or dtype
+        if self.kv_dtype == torch.uint8:
+            if getattr(model, "cache_layout", lambda: None)() is not None:
+                raise ValueError(f"--kv-cache-dtype fp4: {mcfg.name} has caches of its own layers' forms")
+            if mcfg.head_dim not in (64, 128):
+                raise ValueError(f"--kv-cache-dtype fp4: heads of 64 or 128, {mcfg.name} has {mcfg.head_dim}")
+            if block_size < 16 or block_size & (block_size - 1):
+                raise ValueError(f"--kv-cache-dtype fp4: block size {block_size} is not a power of two from 16 on")
         self.kv_scales = kv_scales
         self.bs = block_size
         self.max_model_len = max_model_len
@@ -203,6 +211,9 @@ class ModelRunner:
             el = torch.tensor([], dtype=self.kv_dtype).element_size()
             return max(1, sum(g * (dk + dv) * self._page_rows(pool) * el
                               for g, dk, dv, pool in map(self._cache_entry, self.cache_layout)))
+        if self.kv_dtype == torch.uint8:
+            return 2 * m.num_local_layers * math.prod(
+                ops.kv4_cache_shape(1, m.local_kv_heads(), self.bs, self.mcfg.head_dim))
         return (2 * m.num_local_layers * m.local_kv_heads() * self.mcfg.head_dim * self.bs *
                 torch.tensor([], dtype=self.kv_dtype).element_size())
 
@@ -316,10 +327,15 @@ class ModelRunner:
             return
         L, nkv, d = m.num_local_layers, m.local_kv_heads(), self.mcfg.head_dim
         # zero-init: stale slots of partially filled blocks must hold finite values
-        self.kv = torch.zeros(L, 2, num_blocks, nkv, self.bs, d, dtype=self.kv_dtype,
-                              device=self.device)
-        self.kv_caches = [(self.kv[l, 0], self.kv[l, 1].view(num_blocks, nkv, self.bs // 8, d, 8))
-                          for l in range(L)]
+        if self.kv_dtype == torch.uint8:
+            self.kv = torch.zeros(L, 2, *ops.kv4_cache_shape(num_blocks, nkv, self.bs, d), dtype=torch.uint8,
+                                  device=self.device)
+            self.kv_caches = [(self.kv[l, 0], self.kv[l, 1]) for l in range(L)]
+        else:
+            self.kv = torch.zeros(L, 2, num_blocks, nkv, self.bs, d, dtype=self.kv_dtype,
+                                  device=self.device)
+            self.kv_caches = [(self.kv[l, 0], self.kv[l, 1].view(num_blocks, nkv, self.bs // 8, d, 8))
+                              for l in range(L)]
         self.num_blocks = num_blocks
         nq = m.layers[0].self_attn.nq if hasattr(m.layers[0], "self_attn") else m.layers[0].qkv_proj.nq
         if self.is_gpu:
@@ -509,7 +525,7 @@ class ModelRunner:
             if self.cache_layout is None:
                 m.decode_workspace = self.workspace
                 nkv = self.model.local_kv_heads()
-                m.decode_grid_z = z if z is not None else ops.decode_grid_z(D, nkv, max_ctx)
+                m.decode_grid_z = z if z is not None else ops.decode_grid_z(D, nkv, max_ctx, cache_dtype=self.kv_dtype)
         elif P and split:
             m.split = self._split_prefill(Tp, P)
         return m
@@ -861,7 +877,7 @@ class ModelRunner:
         torch.cuda.synchronize()
         self.graph_pool = torch.cuda.graph_pool_handle()
         for B, bound in [(B, b) for B in sorted(self.buckets, reverse=True) for b in (*self._short_bounds(B), 0)]:
-            z = ops.decode_grid_z(B, nkv, self.max_model_len, capacity=True)
+            z = ops.decode_grid_z(B, nkv, self.max_model_len, capacity=True, cache_dtype=self.kv_dtype)
             meta = self._meta(B, 0, 0, B, 0, bound or self.max_model_len, z=z)
 
             def step_body(B=B, meta=meta):

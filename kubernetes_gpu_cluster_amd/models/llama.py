@@ -123,8 +123,8 @@ class LlamaAttention(nn.Module):
             return o.view(o.shape[0], self.nq * self.cfg.head_dim)
         if row_scale is not None:
             qkv = self._scaled_rows(qkv, row_scale, self.qkv_proj.weight.dtype)
-        if (_prefill_rope_fused and qkv.is_cuda and qkv.dim() == 2 and m.num_prefill_tokens
-                and not m.num_decodes and self.q_norm is None and self.k_norm is None
+        if (_prefill_rope_fused and qkv.is_cuda and kc.dtype != torch.uint8 and qkv.dim() == 2
+                and m.num_prefill_tokens and not m.num_decodes and self.q_norm is None and self.k_norm is None
                 and m.num_prefill_tokens == qkv.shape[0]):
             ops.kv_write_rope(qkv, positions, ctx.cos_sin, kc, vc, m.slot_mapping, self.nq,
                               self.nkv, self.cfg.head_dim, k_scale=ctx.k_scale,

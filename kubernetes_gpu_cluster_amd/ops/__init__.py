@@ -138,23 +138,48 @@ def rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Ten
                   q_norm_w: Optional[torch.Tensor] = None,
                   k_norm_w: Optional[torch.Tensor] = None, eps: float = 1e-6,
                   use_rope: bool = True, k_scale: float = 1.0,
-                  v_scale: float = 1.0, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+                  v_scale: float = 1.0, dtype: Optional[torch.dtype] = None,
+                  sections: Optional[Sequence[int]] = None) -> torch.Tensor:
     """k_cache / v_cache may be fp8 (torch.float8_e4m3fn): values are stored as
-    fp8(x / scale).  On the GPU ``qkv`` may also be the K9m split-K slices of the QKV
+    fp8(x / scale); or 4-bit (uint8, ``kv4_cache_shape``): blocks of 32 elements of a head have a
+    power of two of their own (k_scale = v_scale = 1), and k is the code nearest to the exactly
+    rotated key.  ``sections``: positions are int64 [A, T], one row per axis (time, height, width),
+    and pair i of a head turns by the axis whose section holds i -- pairs per axis, one after the
+    other, head_dim / 2 in all, 4 axes at most; positions outside ``cos_sin`` take its nearest row.
+    On the GPU ``qkv`` may also be the K9m split-K slices of the QKV
     projection (fp32 [S, T, N], ops/gemm.py linear_qkv): the kernel sums them, and
     ``dtype`` names the activation dtype of q."""
     if not _gpu(qkv):
         return ref.rope_qk_kv_write(qkv, positions, cos_sin, k_cache, v_cache, slot_mapping,
                                     num_heads, num_kv_heads, head_dim, q_norm_w, k_norm_w, eps,
-                                    use_rope, k_scale, v_scale)
+                                    use_rope, k_scale, v_scale, sections)
     sl = qkv.dim() == 3
     T = qkv.shape[1] if sl else qkv.shape[0]
     q = torch.empty(T, num_heads, head_dim, dtype=(dtype or qkv.dtype) if sl else qkv.dtype,
                     device=qkv.device)
     _k().rope_kv_write(qkv, positions, cos_sin, q, k_cache, v_cache, slot_mapping, q_norm_w,
                        k_norm_w, num_heads, num_kv_heads, head_dim, eps, use_rope, k_scale,
-                       v_scale)
+                       v_scale, None if sections is None else list(sections))
     return q
+
+
+def kv4_cache_shape(num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int) -> tuple:
+    """Shape of a 4-bit k_cache or v_cache (uint8, both alike): 4.25 bits an element.  A kv head's page
+    is block_size rows of head_dim / 2 bytes, then their block_size * head_dim / 32 scales
+    (``reference.kv4_parts`` has views of both)."""
+    if head_dim not in (64, 128):
+        raise ValueError(f"4-bit cache: head_dim must be 64 or 128, got {head_dim}")
+    return num_blocks, num_kv_heads, block_size, ref.kv4_row_bytes(head_dim)
+
+
+def kv4_read(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """The values [n, nkv, d] that a 4-bit k_cache or v_cache holds in ``slots`` [n] int64 (every one of
+    them is a number of the ``dtype`` it was written from); slots outside the pool give zeros."""
+    if not _gpu(cache):
+        return ref.kv4_read(cache, slots, dtype)
+    out = torch.empty(slots.shape[0], cache.shape[1], ref.kv4_head_dim(cache), dtype=dtype, device=cache.device)
+    _k().kv4_read(out, cache, slots)
+    return out
 
 
 def kv_write_rope(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
@@ -222,8 +247,11 @@ def _decode_z_cap(ws, B: int, nq: int) -> int:
     return max(1, min(1024, ws[0].numel() // max(1, B * nq)))
 
 
+KV4_TARGET_WAVES = 2048      # 4-bit decode: 8 resident waves per CU
+
+
 def decode_grid_z(batch: int, num_kv_heads: int, max_ctx: int, target_waves: int = 0,
-                  capacity: bool = False) -> int:
+                  capacity: bool = False, cache_dtype: Optional[torch.dtype] = None) -> int:
     """z-slices of the decode grid: enough waves to fill 256 CUs, bounded by the
     context (K1w: two 32-token chunks per wave; 4-wave kernel: 64-token partitions) and by
     the 1024 slices the reduce kernel merges.  Z == 1 (large batches, short contexts) lets the kernel
@@ -236,8 +264,12 @@ def decode_grid_z(batch: int, num_kv_heads: int, max_ctx: int, target_waves: int
     with them 56 pairs x 200, 3000 tokens 8.7 -> 9.2, 21.4 -> 22.5, 48 x 4000 22.6 -> 23.8 (fp8 20.2 -> 21.9).
     ``capacity``: max_ctx is what the rows may come to (a captured graph).  Empty slices cost too, so that the 4-wave
     kernel has no more there than are as fast for short rows: 56 pairs, 32 slices instead of the 19 of 8192 tokens, 40, 500
-    tokens 11.9 -> 13.5, 15.0 -> 17.5; 8 instead of 3 of 544 8.8 -> 9.5, 15.5 -> 12.5 (4: 8.8, 11.7)."""
+    tokens 11.9 -> 13.5, 15.0 -> 17.5; 8 instead of 3 of 544 8.8 -> 9.5, 15.5 -> 12.5 (4: 8.8, 11.7).
+    ``cache_dtype`` uint8: the 4-bit cache, whose kernel is one wave per slice at any size."""
     pairs = max(1, batch * num_kv_heads)
+    if cache_dtype == torch.uint8:
+        chunks = max(1, math.ceil(max_ctx / DECODE_CHUNK))
+        return max(1, min(math.ceil((target_waves or KV4_TARGET_WAVES) / pairs), math.ceil(chunks / 2), 1024))
     if decode_uses_wave(batch, num_kv_heads):
         chunks = max(1, math.ceil(max_ctx / DECODE_CHUNK))
         if not target_waves and chunks <= (10 if pairs >= DECODE_LONG_PAIRS else 4):
@@ -306,6 +338,14 @@ def paged_attention_decode_rope(qkv: torch.Tensor, positions: torch.Tensor,
         return ref.paged_attention_decode(q, k_cache, v_cache, block_tables, context_lens, scale,
                                           k_scale, v_scale)
     sl = qkv.dim() == 3
+    if k_cache.dtype == torch.uint8:          # two launches: a 4-bit block's scale is of lanes the decode kernel has elsewhere
+        t = (dtype or qkv.dtype) if sl else qkv.dtype
+        if row_scale is not None:
+            qkv = ((qkv.sum(0) if sl else qkv.float()) * row_scale[:, None]).to(t)
+        q = rope_kv_write(qkv, positions, cos_sin, k_cache, v_cache, slot_mapping, num_heads, num_kv_heads,
+                          head_dim, q_norm_w, k_norm_w, eps, use_rope, k_scale, v_scale, t)
+        return paged_attention_decode(q, k_cache, v_cache, block_tables, context_lens, scale, workspace, grid_z,
+                                      k_scale=k_scale, v_scale=v_scale)
     B = qkv.shape[1] if sl else qkv.shape[0]
     out = torch.empty(B, num_heads, head_dim, dtype=(dtype or qkv.dtype) if sl else qkv.dtype,
                       device=qkv.device)
@@ -470,7 +510,7 @@ def sample_vp_finish(packed: torch.Tensor, out: Optional[torch.Tensor] = None) -
 
 __all__ = ["load_extension", "rms_norm", "fused_add_rms_norm", "layer_norm", "silu_mul",
            "rope_kv_write", "paged_attention_decode", "paged_attention_decode_rope", "prefill_attention", "sample", "sample_vp_partial", "sample_vp_finish",
-           "decode_partials", "decode_grid_z", "moe_pack", "moe_packable", "prefill_work_list", "ref"]
+           "decode_partials", "decode_grid_z", "kv4_cache_shape", "kv4_read", "moe_pack", "moe_packable", "prefill_work_list", "ref"]
 
 
 # ------------------------------------------------------------------ MoE (K13 / K14)

@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import math
 import struct
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -82,16 +82,30 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor) 
     return torch.cat([x1 * cos - x2 * sin, x2 * cos + x1 * sin], dim=-1).to(x.dtype)
 
 
+def axes_cos_sin(positions: torch.Tensor, cos_sin: torch.Tensor,
+                 sections: Optional[Sequence[int]]) -> tuple[torch.Tensor, torch.Tensor]:
+    """cos, sin [T, d/2] of positions [T], or of [A, T] where axis a turns the pairs of its section
+    (positions outside the table: its nearest row)."""
+    half = cos_sin.shape[1] // 2
+    if sections is None:
+        return cos_sin[positions].chunk(2, dim=-1)
+    axis = torch.repeat_interleave(torch.arange(len(sections)), torch.tensor(list(sections))).to(positions.device)
+    at = positions.clamp(0, cos_sin.shape[0] - 1).t()[:, axis]
+    i = torch.arange(half, device=positions.device)
+    return cos_sin[at, i], cos_sin[at, i + half]
+
+
 def rope_qk_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
                      k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor,
                      num_heads: int, num_kv_heads: int, head_dim: int,
                      q_norm_w: Optional[torch.Tensor] = None,
                      k_norm_w: Optional[torch.Tensor] = None, eps: float = 1e-6,
-                     use_rope: bool = True, k_scale: float = 1.0,
-                     v_scale: float = 1.0) -> torch.Tensor:
+                     use_rope: bool = True, k_scale: float = 1.0, v_scale: float = 1.0,
+                     sections: Optional[Sequence[int]] = None) -> torch.Tensor:
     """K3+K5(+K6): split fused qkv [T, (nq+2nkv)*d], optional per-head q/k RMSNorm,
     RoPE on q,k, scatter k,v into the paged cache at slot_mapping (-1 = skip).
-    Returns rotated q as a contiguous [T, nq, d] tensor."""
+    Returns rotated q as a contiguous [T, nq, d] tensor.  A 4-bit cache (uint8) has the codes
+    nearest to the exactly rotated k."""
     T = qkv.shape[0]
     qs, ks = num_heads * head_dim, num_kv_heads * head_dim
     q = qkv[:, :qs].reshape(T, num_heads, head_dim)
@@ -100,9 +114,21 @@ def rope_qk_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.
     if q_norm_w is not None:
         q = rms_norm(q, q_norm_w, eps)
         k = rms_norm(k, k_norm_w, eps)
-    if use_rope:
+    kv4 = k_cache.dtype == torch.uint8
+    if use_rope and (kv4 or sections is not None):
+        cos, sin = (c.unsqueeze(1) for c in axes_cos_sin(positions, cos_sin, sections))
+
+        def turn(x, t):
+            a, b = x.to(t).chunk(2, dim=-1)
+            return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
+        q = turn(q, torch.float32).to(qkv.dtype)
+        k = turn(k, torch.float64) if kv4 else turn(k, torch.float32).to(qkv.dtype)
+    elif use_rope:
         q = apply_rope(q, positions, cos_sin)
         k = apply_rope(k, positions, cos_sin)
+    if kv4:
+        kv4_cache_write(k, v, k_cache, v_cache, slot_mapping, qkv.dtype)
+        return q.contiguous()
     kv_cache_write(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale)
     return q.contiguous()
 
@@ -133,9 +159,77 @@ def kv_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
     v_cache[blk, :, off // 8, :, off % 8] = to_cache(v[valid].to(v.dtype), v_cache.dtype, v_scale)
 
 
+# ---- the cache in 4 bits: uint8 [nb, nkv, bs, d/2 + d/32]; a kv head's page is its bs rows of d/2
+# bytes (e2m1, even element in the low half), then their bs * d/32 scales (exponent + 127)
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def kv4_row_bytes(d: int) -> int:
+    return d // 2 + d // 32
+
+
+def kv4_head_dim(cache: torch.Tensor) -> int:
+    return cache.shape[3] * 32 // 17
+
+
+def kv4_parts(cache: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Views of a 4-bit cache: numbers [nb, nkv, bs, d/2], scales [nb, nkv, bs, d/32]."""
+    bs, d = cache.shape[2], kv4_head_dim(cache)
+    flat = cache.view(cache.shape[0], cache.shape[1], -1)
+    return (flat[..., :bs * d // 2].unflatten(-1, (bs, d // 2)),
+            flat[..., bs * d // 2:].unflatten(-1, (bs, d // 32)))
+
+
+def kv4_quantize(x: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """Bytes [.., d/2] and scale bytes [.., d/32] of x [.., d]: blocks of 32, whose scale is the power
+    of two under which the largest magnitude is at most 7; e2m1 numbers, ties to the even code, what
+    is over 6 scales is 6, NaN is 0.  The exponent stays where all values are numbers of ``dtype``."""
+    x = x if x.dtype == torch.float64 else x.float()
+    x = torch.where(x == x, x, 0).clamp(torch.finfo(torch.float32).min, torch.finfo(torch.float32).max)
+    b = x.unflatten(-1, (-1, 32))
+    most = b.abs().amax(-1)
+    m, e = torch.frexp(most)
+    lo, hi = (-22, 13) if dtype == torch.float16 else (-120, 125)
+    e = torch.where(most > 0, (e - 3 + (m > 0.875)).clamp(lo, hi), lo)
+    a = torch.ldexp(b, -e.unsqueeze(-1)).abs()
+    code = ((a > 0.25).to(torch.uint8) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) +
+            (a >= 3.5) + (a > 5))
+    code = (code | (b < 0).to(torch.uint8) << 3).flatten(-2).unflatten(-1, (-1, 2))
+    return code[..., 0] | code[..., 1] << 4, (e + 127).to(torch.uint8)
+
+
+def kv4_dequantize(numbers: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """fp32 values [.., d] of bytes [.., d/2] and scale bytes [.., d/32]."""
+    lut = torch.tensor(E2M1 + tuple(-v for v in E2M1), device=numbers.device)
+    v = lut[torch.stack([numbers & 15, numbers >> 4], dim=-1).flatten(-2).long()]
+    return torch.ldexp(v.unflatten(-1, (-1, 32)), scales.int().unsqueeze(-1) - 127).flatten(-2)
+
+
+def kv4_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    slot_mapping: torch.Tensor, dtype: torch.dtype) -> None:
+    bs = k_cache.shape[2]
+    there = (slot_mapping >= 0) & (slot_mapping < k_cache.shape[0] * bs)
+    blk, off = slot_mapping[there] // bs, slot_mapping[there] % bs
+    for x, cache in ((k, k_cache), (v, v_cache)):
+        for part, new in zip(kv4_parts(cache), kv4_quantize(x[there], dtype)):
+            part[blk, :, off] = new
+
+
+def kv4_read(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    bs = cache.shape[2]
+    there = (slots >= 0) & (slots < cache.shape[0] * bs)
+    at = torch.where(there, slots, 0)
+    n, s = (p[at // bs, :, at % bs] for p in kv4_parts(cache))
+    return torch.where(there[:, None, None], kv4_dequantize(n, s), 0).to(dtype)
+
+
 # ---------------------------------------------------------------- attention
 def _gather_kv(k_cache, v_cache, block_table, ctx_len, k_scale=1.0, v_scale=1.0):
     bs = k_cache.shape[2]
+    if k_cache.dtype == torch.uint8:
+        blocks = block_table[:(ctx_len + bs - 1) // bs].long()
+        return tuple(kv4_dequantize(*(p[blocks] for p in kv4_parts(c))).transpose(1, 2).flatten(0, 1)[:ctx_len]
+                     for c in (k_cache, v_cache))
     nb = (ctx_len + bs - 1) // bs
     blocks = block_table[:nb].long()
     k = k_cache[blocks]                                   # [nb, nkv, bs, d]

@@ -1,0 +1,427 @@
+"""The 4-bit cache's kernels (csrc/kernels/kv4_*.hip) and rotary positions on several axes against 64 bits."""
+import pytest
+import torch
+
+import kv4_oracle as oracle
+from kubernetes_gpu_cluster_amd import ops
+from kubernetes_gpu_cluster_amd.ops import reference as ref
+
+pytestmark = pytest.mark.gpu
+
+DT = [torch.bfloat16, torch.float16]
+
+
+def _gen(seed=0):
+    return torch.Generator().manual_seed(seed)
+
+
+def _check_rows(got, want, u, size):
+    """fp32 products and sum of two terms of at most ``size`` (3 roundings each 2^-24 relative of 2 size), then
+    one rounding to the type (or its smallest step, fp16's 2^-25)."""
+    tol = u * 1.01 * want.abs() + 6 * 2.0 ** -24 * size + 2.0 ** -25
+    assert ((got.double() - want).abs() <= tol).all()
+
+
+# ------------------------------------------------------------------ write
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("nq,nkv,d,bs", [(32, 8, 128, 32), (5, 1, 64, 16), (3, 3, 128, 64), (12, 12, 64, 32)])
+@pytest.mark.parametrize("T,sections,slices", [(1, None, 0), (133, None, 0), (133, (10, 9, -1), 0), (37, None, 3),
+                                               (37, (8, 8, 8, -1), 2), (300, (-1,), 0)])
+def test_write(gpu, dt, nq, nkv, d, bs, T, sections, slices):
+    g = _gen(T + d)
+    if sections:
+        sections = [n if n >= 0 else d // 2 - sum(n for n in sections if n >= 0) for n in sections]
+    nb = -(-T // bs) + 2
+    kc = oracle.random_cache(g, nb, nkv, bs, d, dt)
+    vc = oracle.random_cache(g, nb, nkv, bs, d, dt)
+    width = (nq + 2 * nkv) * d
+    x = torch.randn(max(slices, 1), T, width, generator=g) * torch.exp(torch.randn(width, generator=g))
+    qkv = x.float() if slices else torch.cat([x[0].to(dt), torch.zeros(T, 16, dtype=dt)], 1)   # rows of a wider matrix
+    slots = torch.randperm(nb * bs, generator=g)[:T]
+    if T > 30:
+        slots[7], slots[T - 1] = -1, nb * bs + 5              # graph padding; beyond the pool
+    table = ref.rope_cos_sin_cache(d, 400, 10000.0)
+    pos = torch.randint(0, 400, (len(sections), T) if sections else (T,), generator=g)
+    kg, vg = kc.to(gpu), vc.to(gpu)
+    q = ops.rope_kv_write(qkv.to(gpu), pos.to(gpu), table.to(gpu), kg, vg, slots.to(gpu), nq, nkv, d, dtype=dt,
+                          sections=sections)
+    # slices are summed in fp32, in order, and rounded to the type
+    rows = qkv[:, :width] if not slices else x[0]
+    for z in range(1, slices):
+        rows = rows + x[z]
+    rows = rows.to(dt).view(T, nq + 2 * nkv, d).double()
+    cos, sin = oracle.cos_sin_rows(table, pos, sections)
+    _check_rows(q.cpu(), oracle.rotate(rows[:, :nq], cos, sin), torch.finfo(dt).eps / 2, 2 * rows.abs().max())
+    k = oracle.nearest(oracle.rotate(rows[:, nq:nq + nkv], cos, sin), dt)[0]
+    v = oracle.nearest(rows[:, nq + nkv:], dt)[0]
+    there = (slots >= 0) & (slots < nb * bs)
+    for got, want, old in ((kg, k, kc), (vg, v, vc)):
+        back = ops.kv4_read(got, slots.to(gpu), dt).cpu()
+        assert torch.equal(back[there].double(), want[there]) and not back[~there].any()
+        for part, was in zip(ref.kv4_parts(got.cpu()), ref.kv4_parts(old)):      # all other bytes as they were
+            part, was = part.transpose(1, 2).flatten(0, 1), was.transpose(1, 2).flatten(0, 1)
+            kept = torch.ones(nb * bs, dtype=torch.bool)
+            kept[slots[there]] = False
+            assert torch.equal(part[kept], was[kept])
+        n, s = (p[slots[there] // bs, :, slots[there] % bs] for p in ref.kv4_parts(got.cpu()))
+        assert torch.equal(ref.kv4_dequantize(n, s).double(), want[there])
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_write_unrotated_and_special(gpu, dt):
+    """Ties, the scales' ends, subnormal blocks, zeros, infinities and NaN."""
+    d, T = 64, 9
+    x = torch.randn(T, 3, d, generator=_gen(5))
+    x[0, :, :32] = torch.tensor([.25, .75, 1.25, 1.75, 2.5, 3.5, 5, 6] * 4)
+    x[1] = -x[0] * 2.0 ** -7
+    x[2, :, 0], x[2, :, 32] = 60000.0, 7.0
+    x[3], x[4] = x[3] * 2.0 ** -20, 0
+    x[5, :, 1] = float("inf")
+    x[6, :, 2], x[6, :, 3] = float("nan"), -float("inf")
+    x[7, :, 0] = 7.0625
+    x = x.to(dt)
+    kc, vc = (torch.zeros(ops.kv4_cache_shape(2, 1, 16, d), dtype=torch.uint8, device=gpu) for _ in range(2))
+    slots = torch.arange(T, device=gpu)
+    table = ref.rope_cos_sin_cache(d, 4, 10000.0).to(gpu)
+    q = ops.rope_kv_write(x.view(T, -1).to(gpu), slots * 0, table, kc, vc, slots, 1, 1, d, use_rope=False)
+    assert torch.equal(q.cpu().nan_to_num(7), x[:, :1].nan_to_num(7))
+    for c, want in ((kc, x[:, 1:2]), (vc, x[:, 2:])):
+        n, s = ref.kv4_quantize(want, dt)
+        for got, w in zip(ref.kv4_parts(c.cpu()), (n, s)):
+            got = got[0, :, :T].transpose(0, 1)
+            if w is n:                                       # (a zero's sign is not kept by all)
+                got, w = ref.kv4_dequantize(got, s), ref.kv4_dequantize(w, s)
+            assert torch.equal(got, w)
+        assert ops.kv4_read(c, slots, dt).isfinite().all()
+
+
+@pytest.mark.parametrize("cache", ["fp4", "auto"])
+@pytest.mark.parametrize("sections", [None, (24, 20, 20)])
+def test_write_with_norms(gpu, cache, sections):
+    """q / k norms: k's codes are within the step of what 64 bits give, for the norm's rounding to the type."""
+    g, dt, nq, nkv, d, T = _gen(6), torch.bfloat16, 8, 2, 128, 50
+    x = torch.randn(T, (nq + 2 * nkv) * d, generator=g).to(dt)
+    qw, kw = (torch.rand(d, generator=g).add(0.5).to(dt) for _ in range(2))
+    table = ref.rope_cos_sin_cache(d, 100, 10000.0)
+    pos = torch.randint(0, 100, (3, T) if sections else (T,), generator=g)
+    shape = ops.kv4_cache_shape(2, nkv, 32, d)
+    kc, vc = ((torch.zeros(shape, dtype=torch.uint8, device=gpu) for _ in range(2)) if cache == "fp4" else
+              (torch.zeros(2, nkv, 32, d, dtype=dt, device=gpu), torch.zeros(2, nkv, 4, d, 8, dtype=dt, device=gpu)))
+    slots = torch.randperm(64, generator=g)[:T]
+    q = ops.rope_kv_write(x.to(gpu), pos.to(gpu), table.to(gpu), kc, vc, slots.to(gpu), nq, nkv, d, qw.to(gpu),
+                          kw.to(gpu), 1e-6, sections=sections)
+    h = x.double().view(T, -1, d)
+    h = h * (h.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    cos, sin = oracle.cos_sin_rows(table, pos, sections)
+    # the norm's result is rounded to the type (2^-8 of each of the two terms) before the rotation
+    qn, kn = h[:, :nq] * qw.double(), h[:, nq:nq + nkv] * kw.double()
+    off = lambda y: (1.01 * 2.0 ** -8 + 2.0 ** -20) * oracle.rotate(y.abs(), cos.abs(), -sin.abs()).abs() + \
+        (1.01 * 2.0 ** -8 + 2.0 ** -20) * oracle.rotate(y.abs(), cos.abs(), sin.abs()).abs()    # noqa: E731
+    want = oracle.rotate(qn, cos, sin)
+    assert ((q.cpu().double() - want).abs() <= off(qn) + 1.01 * 2.0 ** -8 * (want.abs() + off(qn))).all()
+    want = oracle.rotate(kn, cos, sin)
+    if cache == "fp4":
+        got = ops.kv4_read(kc, slots.to(gpu), dt).cpu().double()
+        e = ref.kv4_parts(kc.cpu())[1][slots // 32, :, slots % 32].double() - 127
+        step = (2 ** e).repeat_interleave(32, -1)            # no number is further than this from its code
+    else:
+        got, step = kc.cpu().double()[slots // 32, :, slots % 32], 1.01 * 2.0 ** -8 * (want.abs() + off(kn))
+    assert ((got - want).abs() <= step + off(kn)).all()
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("cache", ["auto", "fp8"])
+@pytest.mark.parametrize("T,sections,slices", [(77, (16, 24, 24), 0), (77, (5, 0, 40, 19), 0), (9, (64,), 2)])
+def test_axes_of_the_wider_caches(gpu, dt, cache, T, sections, slices):
+    g, nq, nkv, d, bs = _gen(7), 8, 2, 128, 16
+    t = torch.float8_e4m3fn if cache == "fp8" else dt
+    mk = lambda: (torch.zeros(8, nkv, bs, d).to(t).to(gpu), torch.zeros(8, nkv, bs // 8, d, 8).to(t).to(gpu))   # noqa: E731
+    x = torch.randn(max(slices, 1), T, (nq + 2 * nkv) * d, generator=g)
+    x = x.to(gpu) if slices else x[0].to(dt).to(gpu)
+    table = ref.rope_cos_sin_cache(d, 90, 10000.0)
+    pos = torch.randint(-5, 99, (len(sections), T), generator=g)
+    slots = torch.randperm(8 * bs, generator=g)[:T].to(gpu)
+    kc, vc = mk()
+    q = ops.rope_kv_write(x, pos.to(gpu), table.to(gpu), kc, vc, slots, nq, nkv, d, dtype=dt, sections=sections)
+    # each pair as the one-position kernel turns it, from a table of that axis's rows
+    for a, n in enumerate(sections):
+        rows = table[pos[a].clamp(0, 89)].contiguous().to(gpu)
+        k2, v2 = mk()
+        q2 = ops.rope_kv_write(x, torch.arange(T, device=gpu), rows, k2, v2, slots, nq, nkv, d, dtype=dt)
+        i = torch.arange(sum(sections[:a]), sum(sections[:a + 1]), device=gpu)
+        i = torch.cat([i, i + d // 2])
+        assert torch.equal(q[..., i], q2[..., i])
+        assert torch.equal(kc.float()[..., i], k2.float()[..., i]) and torch.equal(vc.float(), v2.float())
+
+
+# ------------------------------------------------------------------ attention
+def _attention_case(seed, nq, nkv, d, bs, dt, new, old, k_size=1.0):
+    g = _gen(seed)
+    totals = [a + b for a, b in zip(new, old)]
+    bt, nb = oracle.tables(g, totals, bs)
+    kc = oracle.random_cache(g, nb, nkv, bs, d, dt, k_size)
+    vc = oracle.random_cache(g, nb, nkv, bs, d, dt)
+    kc[0], vc[0] = 255, 255                                   # nobody's page: no finite value
+    for c in (kc, vc):                                        # and behind the last tokens
+        for i, n in enumerate(totals):
+            if n % bs:
+                for p in ref.kv4_parts(c):
+                    p[bt[i, n // bs], :, n % bs:] = 255
+    q = torch.randn(sum(new), nq, d, generator=g).to(dt)
+    return q, kc, vc, bt, totals
+
+
+def _check_attention(got, q, kc, vc, bt, new, totals, scale):
+    nq, nkv, d = q.shape[1], kc.shape[1], q.shape[2]
+    at = 0
+    for i, (m, n) in enumerate(zip(new, totals)):
+        if n == 0:
+            assert not got[at:at + m].any()
+            at += m
+            continue
+        seen = torch.arange(n)[None] <= torch.arange(n - m, n)[:, None]
+        for h in range(nkv):
+            k, v = (oracle.rows(c, bt[i], n, h, d) for c in (kc, vc))
+            for j in range(h * (nq // nkv), (h + 1) * (nq // nkv)):
+                o, tol = oracle.attend(q[at:at + m, j], k, v, scale, seen, q.dtype)
+                off = (got[at:at + m, j].double() - o).abs()
+                assert (off <= tol).all(), (i, j, float((off / tol).max()))
+        at += m
+
+
+DECODE = [
+    # q heads, kv heads, head, page, contexts
+    (4, 1, 128, 32, [0, 1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 100]),
+    (32, 8, 128, 32, [640, 1, 0, 333]),
+    (12, 12, 64, 16, [47, 200, 1]),
+    (16, 1, 64, 64, [129, 5]),
+    (8, 8, 128, 16, [1500]),
+    (10, 2, 64, 32, [500, 31, 96]),
+    (7, 1, 128, 128, [257, 128]),
+]
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("nq,nkv,d,bs,ctx", DECODE)
+@pytest.mark.parametrize("z", [1, 2, 3, 0, 64])
+def test_decode(gpu, dt, nq, nkv, d, bs, ctx, z):
+    q, kc, vc, bt, _ = _attention_case(sum(ctx), nq, nkv, d, bs, dt, [1] * len(ctx), [c - 1 for c in ctx])
+    ws = ops.decode_partials(len(ctx), nq, d, 64 * 64 // bs, bs, gpu)
+    for t in ws:
+        t.fill_(float("nan"))                                 # no slice is read that none wrote
+    z = z or ops.decode_grid_z(len(ctx), nkv, max(ctx), cache_dtype=torch.uint8)
+    out = torch.full_like(q, 7).to(gpu)
+    got = ops.paged_attention_decode(q.to(gpu), kc.to(gpu), vc.to(gpu), bt.to(gpu),
+                                     torch.tensor(ctx, dtype=torch.int32, device=gpu), d ** -0.5, ws, z, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    _check_attention(got.cpu(), q, kc, vc, bt, [1] * len(ctx), ctx, d ** -0.5)
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_decode_sharp_rows(gpu, dt):
+    """Keys large enough that one token has all the weight, and scores far apart between slices."""
+    ctx = [700, 90, 33]
+    q, kc, vc, bt, _ = _attention_case(3, 8, 2, 128, 32, dt, [1] * 3, [c - 1 for c in ctx], k_size=32.0)
+    for z in (1, 4, 11):
+        got = ops.paged_attention_decode(q.to(gpu), kc.to(gpu), vc.to(gpu), bt.to(gpu),
+                                         torch.tensor(ctx, dtype=torch.int32, device=gpu), 0.25, None, z)
+        _check_attention(got.cpu(), q, kc, vc, bt, [1] * 3, ctx, 0.25)
+
+
+PROMPTS = [
+    # q heads, kv heads, head, page, new rows, cached before
+    (4, 1, 128, 32, [1, 2, 31, 32, 33, 64, 65], [0, 0, 0, 0, 0, 0, 0]),
+    (32, 8, 128, 32, [130, 1, 257], [0, 63, 100]),
+    (12, 12, 64, 16, [128, 3, 47], [16, 15, 17]),
+    (2, 1, 128, 64, [200], [5]),
+    (6, 2, 64, 32, [129, 64], [700, 0]),
+    (16, 1, 128, 16, [33, 90], [31, 1]),
+    (7, 1, 64, 32, [300], [0]),
+    (1, 1, 128, 32, [1, 1, 1], [0, 64, 255]),
+]
+
+
+def _starts(new):
+    return torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("nq,nkv,d,bs,new,old", PROMPTS)
+def test_prompts(gpu, dt, nq, nkv, d, bs, new, old):
+    q, kc, vc, bt, totals = _attention_case(sum(new), nq, nkv, d, bs, dt, new, old)
+    qg = torch.cat([q, torch.zeros(3, nq, d, dtype=dt)]).to(gpu)
+    out = torch.full_like(qg, 7)                              # rows behind the last sequence: as they were
+    got = ops.prefill_attention(qg, kc.to(gpu), vc.to(gpu), bt.to(gpu), _starts(new).to(gpu),
+                                torch.tensor(totals, dtype=torch.int32, device=gpu), d ** -0.5, out=out)
+    assert got.data_ptr() == out.data_ptr() and (out[-3:] == 7).all()
+    _check_attention(got[:-3].cpu(), q, kc, vc, bt, new, totals, d ** -0.5)
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_prompts_sharp_rows(gpu, dt):
+    new, old = [150, 40], [90, 0]
+    q, kc, vc, bt, totals = _attention_case(11, 8, 2, 128, 32, dt, new, old, k_size=32.0)
+    got = ops.prefill_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), bt.to(gpu), _starts(new).to(gpu),
+                                torch.tensor(totals, dtype=torch.int32, device=gpu), 0.25)
+    _check_attention(got.cpu(), q, kc, vc, bt, new, totals, 0.25)
+
+
+def test_empty_calls(gpu):
+    kc = torch.zeros(ops.kv4_cache_shape(3, 2, 16, 64), dtype=torch.uint8, device=gpu)
+    i32 = lambda *n: torch.zeros(*n, dtype=torch.int32, device=gpu)   # noqa: E731
+    q = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device=gpu)
+    assert ops.paged_attention_decode(q, kc, kc, i32(0, 2), i32(0), 1.0).shape == q.shape
+    assert ops.prefill_attention(q, kc, kc, i32(1, 2), i32(2), i32(1), 1.0).shape == q.shape
+    table = torch.zeros(4, 64, device=gpu)
+    none = torch.zeros(0, dtype=torch.int64, device=gpu)
+    assert ops.rope_kv_write(torch.zeros(0, 512, dtype=torch.bfloat16, device=gpu), none, table, kc, kc.clone(), none,
+                             4, 2, 64).shape == q.shape
+    assert ops.kv4_read(kc, none, torch.float16).shape == (0, 2, 64)
+
+
+# ------------------------------------------------------------------ together
+def _prompt_then_decode(dev, dt, graph):
+    """A prompt in two chunks, then decode steps, as the engine calls the operators; positions on three axes.
+    -> attention results, on the CPU."""
+    g, nq, nkv, d, bs, n = _gen(21), 8, 2, 128, 32, 75
+    shape = ops.kv4_cache_shape(5, nkv, bs, d)
+    kc, vc = (torch.zeros(shape, dtype=torch.uint8, device=dev) for _ in range(2))
+    table = ref.rope_cos_sin_cache(d, 128, 10000.0).to(dev)
+    bt = torch.tensor([[3, 1, 4, 0]], dtype=torch.int32, device=dev)
+    x = torch.randn(n + 6, (nq + 2 * nkv) * d, generator=g).to(dt).to(dev)
+    pos = torch.stack([torch.arange(n + 6), torch.arange(n + 6) // 2, torch.arange(n + 6) % 7]).to(dev)
+    slots = (bt[0].long()[torch.arange(n + 6, device=dev) // bs] * bs + torch.arange(n + 6, device=dev) % bs)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)   # noqa: E731
+    sec, out = (16, 24, 24), []
+    for a, b in ((0, 40), (40, n)):
+        q = ops.rope_kv_write(x[a:b], pos[:, a:b], table, kc, vc, slots[a:b], nq, nkv, d, sections=sec)
+        out.append(ops.prefill_attention(q, kc, vc, bt, i32(0, b - a), i32(b), d ** -0.5))
+    ws = ops.decode_partials(1, nq, d, 4, bs, dev) if graph else None
+    row, at, slot, length = x[:1].clone(), pos[:, :1].clone(), slots[:1].clone(), i32(0)
+
+    def step():
+        q = ops.rope_kv_write(row, at, table, kc, vc, slot, nq, nkv, d, sections=sec)
+        return ops.paged_attention_decode(q, kc, vc, bt, length, d ** -0.5, ws, 2)
+    run = None
+    for t in range(n, n + 6):
+        row.copy_(x[t:t + 1]), at.copy_(pos[:, t:t + 1]), slot.copy_(slots[t:t + 1]), length.fill_(t + 1)
+        if graph and run is None:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                step()
+            torch.cuda.current_stream().wait_stream(side)
+            run = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(run):
+                held = step()
+        if graph:
+            run.replay()
+            out.append(held.clone())
+            torch.cuda.synchronize()
+        else:
+            out.append(step())
+    return [o.cpu() for o in out], kc.cpu(), vc.cpu()
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_prompt_then_decode(gpu, dt):
+    """The same run eagerly, with decode steps as replays of one captured graph, and on the CPU: equal caches; and
+    results, to the type's rounding, of the CPU's."""
+    eager, kc, vc = _prompt_then_decode(gpu, dt, False)
+    graph, kc2, vc2 = _prompt_then_decode(gpu, dt, True)
+    cpu, kc3, vc3 = _prompt_then_decode(torch.device("cpu"), dt, False)
+    assert torch.equal(kc, kc2) and torch.equal(vc, vc2)
+    for a, b in ((kc, kc3), (vc, vc3)):
+        (n, s), (m, r) = ref.kv4_parts(a), ref.kv4_parts(b)
+        used = [3, 1, 4]
+        assert torch.equal(ref.kv4_dequantize(n[used], s[used]), ref.kv4_dequantize(m[used], r[used]))
+    for a, b, c in zip(eager, graph, cpu):
+        assert torch.equal(a, b)
+        # two roundings of probabilities' products and results on one side, one on the other, of values below 8
+        assert ((a.double() - c.double()).abs() <= 3 * torch.finfo(dt).eps * 8).all()
+
+
+def test_on_another_stream(gpu):
+    """Work on a stream that is not the default one, behind work that it waits for."""
+    q, kc, vc, bt, totals = _attention_case(5, 8, 2, 128, 32, torch.bfloat16, [1] * 4, [600, 31, 32, 5])
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        a = [t.to(gpu, non_blocking=True) for t in (q, kc, vc, bt, torch.tensor(totals, dtype=torch.int32))]
+        got = ops.paged_attention_decode(*a, 128 ** -0.5, None, 4)
+    side.synchronize()
+    _check_attention(got.cpu(), q, kc, vc, bt, [1] * 4, totals, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("model", ["tiny-llama", "tiny-qwen3"])
+def test_engine(gpu, model):
+    """--kv-cache-dtype fp4 through the engine: decode by graphs and eagerly give the same greedy tokens, and first
+    tokens are among the five likeliest of the 16-bit cache's run."""
+    from kubernetes_gpu_cluster_amd.engine.llm_engine import LLM
+    from kubernetes_gpu_cluster_amd.engine.sequence import SamplingParams
+    prompts = [[5 + i, 6, 7, 8, 9] * 9 for i in range(3)]
+    sp = SamplingParams(temperature=0, max_tokens=12, ignore_eos=True, logprobs=5)
+    outs = []
+    for kvd, eager in (("auto", False), ("fp4", False), ("fp4", True)):
+        llm = LLM(model, device="cuda", dtype="bfloat16", random_init=True, seed=2, max_model_len=256, max_num_seqs=4,
+                  max_num_batched_tokens=64, kv_cache_dtype=kvd, enforce_eager=eager)
+        r = llm.engine.executor.runner
+        if kvd == "fp4":
+            assert r.kv.dtype == torch.uint8
+        outs.append(llm.generate(prompts, sp))
+        assert (r.stats["graph_steps"] > 0) == (not eager)
+        llm.shutdown()
+    for a, b in zip(outs[0], outs[1]):
+        assert b.logprobs[0][0] in [t for t, _ in a.logprobs[0][2]]
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals(gpu):
+    bf, d = torch.bfloat16, 128
+    kc = torch.zeros(ops.kv4_cache_shape(4, 2, 16, d), dtype=torch.uint8, device=gpu)
+    q = torch.zeros(3, 4, d, dtype=bf, device=gpu)
+    bt = torch.zeros(3, 2, dtype=torch.int32, device=gpu)
+    n = torch.ones(3, dtype=torch.int32, device=gpu)
+    table = torch.zeros(8, d, device=gpu)
+    x = torch.zeros(3, 8 * d, dtype=bf, device=gpu)
+    pos = torch.zeros(3, dtype=torch.int64, device=gpu)
+
+    def no(what, f, *a, **k):
+        with pytest.raises((RuntimeError, ValueError), match=what):
+            f(*a, **k)
+    dec, pre, wr = ops.paged_attention_decode, ops.prefill_attention, ops.rope_kv_write
+    no("own scales", dec, q, kc, kc, bt, n, 1.0, k_scale=0.5)
+    no("own scales", pre, q, kc, kc, bt[:1], n[:2], n[:1], 1.0, v_scale=2.0)
+    no("own scales", wr, x, pos, table, kc, kc, pos, 4, 2, d, k_scale=0.5)
+    no("dtype mismatch", dec, q, kc, kc.view(torch.int8), bt, n, 1.0)
+    no("contiguous", dec, q, kc[:, :, :, :60], kc[:, :, :, :60], bt, n, 1.0)
+    no("contiguous", dec, q, kc.transpose(0, 1), kc.transpose(0, 1), bt, n, 1.0)
+    no("4-bit cache", dec, q[:, :, :64].contiguous(), kc, kc, bt, n, 1.0)
+    no("bf16/f16", dec, q.float(), kc, kc, bt, n, 1.0)
+    no("block_size", dec, q, kc[:, :, :8].contiguous(), kc[:, :, :8].contiguous(), bt, n, 1.0)
+    odd = torch.zeros(ops.kv4_cache_shape(4, 2, 24, d), dtype=torch.uint8, device=gpu)
+    no("power of two", dec, q, odd, odd, bt, n, 1.0)
+    no("GQA", dec, torch.zeros(3, 34, d, dtype=bf, device=gpu), kc, kc, bt, n, 1.0)
+    no("GQA", dec, torch.zeros(3, 3, d, dtype=bf, device=gpu), kc, kc, bt, n, 1.0)
+    no("block_tables", dec, q, kc, kc, bt.long(), n, 1.0)
+    no("block_tables", dec, q, kc, kc, bt[:2], n, 1.0)
+    no("ctx_lens", dec, q, kc, kc, bt, n[:2], 1.0)
+    no("different device", dec, q, kc, kc, bt.cpu(), n, 1.0)
+    no("different device", dec, q, kc, kc.cpu(), bt, n, 1.0)
+    no("query_start_loc", pre, q, kc, kc, bt[:1], n, n[:1], 1.0, n, n)
+    no("seq_lens", pre, q, kc, kc, bt[:2], n, n[:1], 1.0, n, n)
+    no("work list", pre, q, kc, kc, bt[:2], n, n[:2], 1.0, n, n[:2])
+    no("head_dim", wr, x, pos, torch.zeros(8, 96, device=gpu), kc, kc, pos, 4, 2, 96)
+    no("positions", wr, x, pos[:2], table, kc, kc, pos, 4, 2, d)
+    no("slot_mapping", wr, x, pos, table, kc, kc, pos[:2], 4, 2, d)
+    no("16-byte", wr, torch.zeros(3 * 8 * d + 4, dtype=bf, device=gpu)[4:].view(3, -1), pos, table, kc, kc, pos, 4, 2, d)
+    p2 = pos.expand(2, 3).contiguous()
+    no("sections of", wr, x, p2, table, kc, kc, pos, 4, 2, d, sections=(30, 30))
+    no("1 to 4", wr, x, pos.expand(5, 3), table, kc, kc, pos, 4, 2, d, sections=(30, 30, 1, 1, 2))
+    no("0 to d / 2", wr, x, p2, table, kc, kc, pos, 4, 2, d, sections=(-1, 65))
+    no(r"\[sections, T\]", wr, x, pos, table, kc, kc, pos, 4, 2, d, sections=(32, 32))
+    no("rotated head", wr, x, p2, table, kc, kc, pos, 4, 2, d, sections=(32, 32), use_rope=False)
+    no("empty cos_sin", wr, x, p2, table[:0], kc, kc, pos, 4, 2, d, sections=(32, 32))
+    no("write q too", ops.kv_write_rope, x, pos, table, kc, kc, pos, 4, 2, d)
+    no("4-D / v_cache 5-D", ops.prefill_attention_rope, x, table, kc, kc, bt[:1], n[:2], n[:1], 1.0, 4, d, n[:1], n[:1])
+    no("slots int64", torch.ops.kgc.kv4_read, torch.zeros(3, 2, d, dtype=bf, device=gpu), kc, pos.int())
+    no("out bf16", torch.ops.kgc.kv4_read, torch.zeros(3, 2, d, device=gpu), kc, pos)
