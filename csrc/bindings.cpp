@@ -458,10 +458,12 @@ void paged_decode_rope(Tensor out, Tensor qkv, Tensor positions, Tensor cos_sin,
 
 void prefill_attention(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables,
                        Tensor query_start_loc, Tensor seq_lens, Tensor work_seq,
-                       Tensor work_mblk, double scale, double k_scale, double v_scale, int64_t max_len) {
+                       Tensor work_mblk, double scale, double k_scale, double v_scale, int64_t max_len,
+                       std::optional<Tensor> partials) {
   check_gpu(q, "q");
   c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
   TORCH_CHECK(q.dim() == 3 && q.is_contiguous(), "q [T, nq, d] contiguous");
+  TORCH_CHECK(!partials.has_value() || k_cache.scalar_type() == at::kByte, "kgc.prefill_attention: partials are for 4-bit caches");
   if (k_cache.scalar_type() == at::kByte) {
     check_kv4_attention(q, out, k_cache, v_cache, block_tables, k_scale, v_scale);
     const int64_t P = block_tables.size(0);
@@ -473,6 +475,17 @@ void prefill_attention(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Ten
     for (const Tensor* t : {&query_start_loc, &seq_lens, &work_seq, &work_mblk}) check_same_dev(q, *t, "prefill operand");
     TORCH_CHECK(work_seq.numel() <= 2147483647 && q.size(1) <= 65535, "grid");
     kgc::Kv4Prefill a{};
+    a.Z = 1;
+    if (partials.has_value()) {
+      const int64_t rows = q.size(0) * q.size(1), each = q.size(2) + 2;
+      check_same_dev(q, *partials, "partials");
+      a.Z = (int)std::min<int64_t>(32, rows > 0 ? partials->numel() / (rows * each) : 1);
+      TORCH_CHECK(partials->scalar_type() == at::kFloat && partials->is_contiguous() && a.Z >= 1,
+                  "kgc.prefill_attention: partials fp32, rows * heads * (d + 2) for each of 1 to 32 slices");
+      aligned16(*partials, "partials");
+      a.part_o = partials->data_ptr<float>();
+      a.part_ml = a.part_o + rows * a.Z * q.size(2);
+    }
     a.q = q.data_ptr();
     a.k_cache = k_cache.data_ptr();
     a.v_cache = v_cache.data_ptr();
@@ -2996,7 +3009,8 @@ TORCH_LIBRARY(kgc, m) {
         "Tensor? row_scale=None) -> ()");
   m.def("prefill_attention(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, "
         "Tensor block_tables, Tensor query_start_loc, Tensor seq_lens, Tensor work_seq, "
-        "Tensor work_mblk, float scale, float k_scale=1.0, float v_scale=1.0, int max_len=0) -> ()");
+        "Tensor work_mblk, float scale, float k_scale=1.0, float v_scale=1.0, int max_len=0, "
+        "Tensor(b!)? partials=None) -> ()");
   m.def("prefill_attention_rope(Tensor(a!) out, Tensor qkv, Tensor cos_sin, Tensor k_cache, "
         "Tensor v_cache, Tensor block_tables, Tensor query_start_loc, Tensor seq_lens, "
         "Tensor work_seq, Tensor work_mblk, int nq, float scale, float k_scale=1.0, "

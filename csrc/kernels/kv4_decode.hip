@@ -1,8 +1,8 @@
 // Paged-attention decode over the 4-bit cache (kv4.h): one query row per sequence.
 //
-// One wave per (sequence, kv head, z-slice), as paged_decode_wave_kernel (attention_decode.hip) and with its slices
-// (decode_slices.h) and its merge.  A chunk is 32 tokens, two groups of 16; a page holds 16 or more, so that a group lies in
-// one.  Lane (token r16 of a group, quarter qd of the head) loads its quarter row with one load of D / 8 bytes, and the
+// A workgroup of NW waves per (sequence, kv head, z-slice), with the slices and the merge of paged_decode_wave_kernel
+// (decode_slices.h, attention_decode.hip); its waves share the slice's chunks and merge in LDS, so that most calls are one
+// launch.  A chunk is 32 tokens, two groups of 16; a page holds 16 or more, so that a group lies in one.  Lane (token r16 of a group, quarter qd of the head) loads its quarter row with one load of D / 8 bytes, and the
 // scale with it; next chunk's loads are on their way while one computes.
 //   S^T[token][head] = K Q^T: the quarter row, widened, is the operand of D / 32 MFMAs as it is -- their contraction takes the
 //                      head's elements in the order (quarter, 8 of it, next 8 ..), and so does q's operand
@@ -22,17 +22,22 @@ __device__ __forceinline__ float kv4_max_rows(float x) {     // over the four la
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(64, 2) void kv4_decode_kernel(
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void kv4_decode_kernel(
     T* __restrict__ out, const T* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
     const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ ctx_lens, float* __restrict__ max_logits,
     float* __restrict__ exp_sums, float* __restrict__ tmp_out, int nq, int nkv, int bs_log2, float scale_log2,
     int num_blocks, DecodeLeast least) {
   typedef typename Vec8<T>::type V8;
   constexpr int KS = D / 32, DT = D / 16, VS = D + 16;       // VS: the 4 rows x 32 bytes of a transposing read on 32 banks
-  __shared__ __attribute__((aligned(16))) T lds_v[32 * VS];
+  constexpr int OS = D + 4;                                  // floats of a head's row where the waves meet
+  static_assert(32 * VS * sizeof(T) >= 16 * OS * sizeof(float), "a wave's results in its own V rows");
+  __shared__ __attribute__((aligned(16))) T all_v[NW][32 * VS];
+  __shared__ float all_m[NW][16], all_l[NW][16];
   const int b = blockIdx.x, h = blockIdx.y, z = blockIdx.z, Z = gridDim.z;
-  const int lane = threadIdx.x, r16 = lane & 15, qd = lane >> 4;
+  const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, r16 = lane & 15, qd = lane >> 4;
+  T* lds_v = all_v[wave];
   const int G = nq / nkv;
   int ctx_in = ctx_lens[b];
   KGC_DCHECK_RANGE(ctx_in, 0, (bt_stride << bs_log2) + 1, "decode ctx_len");
@@ -45,7 +50,9 @@ __global__ __launch_bounds__(64, 2) void kv4_decode_kernel(
   const int min_per = decode_min_chunks(least, nchunk);
   const int per = decode_slice_chunks(nchunk, Z, min_per);
   const int nused = decode_used_slices(nchunk, Z, min_per);
-  const int c0 = min(nchunk, z * per), c1 = min(nchunk, c0 + per);
+  const int s0 = min(nchunk, z * per), s1 = min(nchunk, s0 + per);
+  if (s0 >= s1 && (z > 0 || nchunk > 0)) return;             // the whole workgroup: an empty slice is not merged
+  const int c0 = s0 + (s1 - s0) * wave / NW, c1 = s0 + (s1 - s0) * (wave + 1) / NW;
   const int end = min(ctx, c1 << 5);                         // this wave's tokens: [32 c0, end)
 
   struct Frag {
@@ -175,8 +182,50 @@ __global__ __launch_bounds__(64, 2) void kv4_decode_kernel(
 
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
+  const bool whole = Z == 1 || nused == 1;  // the merge skips such a row
+  if constexpr (NW > 1) {
+    float* mine = reinterpret_cast<float*>(lds_v);
+#pragma unroll
+    for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(mine + r16 * OS + 16 * t + 4 * qd) = o[t];
+    if (qd == 0) {
+      all_m[wave][r16] = m_run;
+      all_l[wave][r16] = l_run;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < G * (D / 4); e += 64 * NW) {
+      const int g = e / (D / 4), d = e % (D / 4) * 4;
+      float top = all_m[0][g];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) top = fmaxf(top, all_m[w][g]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float f = __builtin_amdgcn_exp2f(all_m[w][g] - ref);
+        acc += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(all_v[w]) + g * OS + d) * f;
+        sum += all_l[w][g] * f;
+      }
+      const int64_t row = (int64_t)b * nq + h * G + g;
+      if (whole) {
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        Pack4<T> pk;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pk.h[i] = from_f<T>(acc[i] * inv);
+        *reinterpret_cast<u32x2*>(out + row * D + d) = pk.u;
+      } else {
+        const int64_t prow = row * Z + z;
+        *reinterpret_cast<f32x4*>(tmp_out + prow * D + d) = acc;
+        if (d == 0) {
+          max_logits[prow] = sum != sum ? INFINITY : top;    // a NaN is the merged row's too
+          exp_sums[prow] = sum;
+        }
+      }
+    }
+    return;
+  }
   const int64_t row = (int64_t)b * nq + h * G + r16;
-  if (Z == 1 || nused == 1) {               // the whole context: the merge skips such a row
+  if (whole) {
     if (z > 0 || r16 >= G) return;
     const float inv = l_run > 0.f || l_run != l_run ? 1.f / l_run : 0.f;
     T* orow = out + row * D + 4 * qd;
@@ -195,28 +244,49 @@ __global__ __launch_bounds__(64, 2) void kv4_decode_kernel(
 #pragma unroll
   for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(dst + 16 * t) = o[t];
   if (qd == 0) {
-    max_logits[prow] = m_run;
+    max_logits[prow] = l_run != l_run ? INFINITY : m_run;
     exp_sums[prow] = l_run;
   }
 }
 
-template <typename T>
-static void kv4_decode_dispatch(const Kv4Decode& a, DecodeLeast least, float sl2, hipStream_t s) {
-#define KGC_KV4_DEC(DD)                                                                                                \
-  kv4_decode_kernel<T, DD><<<dim3(a.B, a.nkv, a.Z), 64, 0, s>>>(                                                         \
+template <typename T, int D>
+static void kv4_decode_dispatch(const Kv4Decode& a, int waves, DecodeLeast least, float sl2, hipStream_t s) {
+#define KGC_KV4_DEC(NW)                                                                                                \
+  kv4_decode_kernel<T, D, NW><<<dim3(a.B, a.nkv, a.Z), 64 * NW, 0, s>>>(                                                         \
       (T*)a.out, (const T*)a.q, (const uint8_t*)a.k_cache, (const uint8_t*)a.v_cache, a.block_tables, a.bt_stride,      \
       a.ctx_lens, a.max_logits, a.exp_sums, a.tmp_out, a.nq, a.nkv, a.bs_log2, sl2, a.num_blocks, least)
-  if (a.D == 128) KGC_KV4_DEC(128);
-  else KGC_KV4_DEC(64);
+  if (waves == 8) KGC_KV4_DEC(8);
+  else if (waves == 4) KGC_KV4_DEC(4);
+  else KGC_KV4_DEC(1);
 #undef KGC_KV4_DEC
 }
 
+// Waves per workgroup (ops/__init__.py has the same numbers, and chooses Z by them).  us, 8 kv heads of 128 unless said, one
+// launch or, with ->, two:
+//   fewer than 64 pairs leave CUs free for slices, and four waves meet sooner than eight: 1 x 128 4.9 (eight 5.7), 1 x 2000 eight slices
+//     -> 7.6 (9.1), 4 x 1000 -> 8.3 (8.9);
+//   up to 512 eight waves take the place of slices: 32 x 2000 16.5 (four 20.5, four and two slices -> 21.1), 33 x 1001 of 12 heads of
+//     64 10.5 (10.8, -> 13.5);
+//   from 512 on the LDS of eight (two workgroups per CU) makes short contexts wait: 64 x 512 10.8 (11.3), 64 x 8192 96.6 (97.2);
+//   from 1024 on a wave has a pair to itself: 256 x 60 8.1 (four 13.1, eight 20.5), 128 x 1000 30.6 (31.6, 32.0), 256 x 640 36.3
+//     (39.0, 47.1); long ones are slower so, 128 x 4000 104 (four 108, eight 95).
+static int kv4_decode_waves(int64_t pairs) { return pairs >= 1024 ? 1 : pairs >= 512 ? 4 : pairs >= 64 ? 8 : 4; }
+
 void launch_kv4_decode(int dtype, const Kv4Decode& a, float scale, hipStream_t s) {
   if (a.B == 0) return;
-  const DecodeLeast least{-1, 2, 2};
+  const int64_t pairs = (int64_t)a.B * a.nkv;
+  const int waves = kv4_decode_waves(pairs);
+  // Slices hold two chunks (the pipeline) for each wave or more, and contexts of up to 16 chunks, 64 from 64 pairs on, are one:
+  // 1 x 500 6.3 us whole, 7.5 as two with their merge; 16 x 2000 13.5 and 13.4.
+  const DecodeLeast least{pairs >= 64 ? 64 : 16, 2 * waves, 2 * waves};
   const float sl2 = scale * 1.4426950408889634f;
-  if (dtype == DT_BF16) kv4_decode_dispatch<bf16>(a, least, sl2, s);
-  else kv4_decode_dispatch<f16>(a, least, sl2, s);
+  if (dtype == DT_BF16) {
+    if (a.D == 128) kv4_decode_dispatch<bf16, 128>(a, waves, least, sl2, s);
+    else kv4_decode_dispatch<bf16, 64>(a, waves, least, sl2, s);
+  } else {
+    if (a.D == 128) kv4_decode_dispatch<f16, 128>(a, waves, least, sl2, s);
+    else kv4_decode_dispatch<f16, 64>(a, waves, least, sl2, s);
+  }
   if (a.Z > 1)
     launch_paged_decode_merge(dtype, a.out, a.max_logits, a.exp_sums, a.tmp_out, a.ctx_lens, a.B, a.nq, a.D, a.Z,
                               a.bt_stride << a.bs_log2, least, s);

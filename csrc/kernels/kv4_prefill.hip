@@ -9,6 +9,9 @@
 // v_mfma_f32_32x32x16: S^T = K Q^T and O^T = V^T P^T, so that a query is a lane's column in every accumulator: its maximum
 // and sum are the lane's own (and its partner's, lane ^ 32), and S^T's accumulator, packed, is the B operand of the second product.
 // V's rows become columns by the transposing LDS read.
+//
+// Z > 1: few rows after long contexts leave CUs idle, so that Z workgroups share an item's tiles; each leaves its rows' maximum,
+// sum and unnormalised result, which kv4_prefill_merge_kernel joins.
 #include "common.h"
 #include "kv4.h"
 #include "launch.h"
@@ -22,31 +25,38 @@ __device__ __forceinline__ float kv4_max_pair(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// Where 16-byte chunk c of a tile's row lies: at c ^ swz(row).  Of K, 16 rows' same chunk is read at a time; of V, 4 rows'
+// four chunks; and 4 rows' same chunk of every quarter is written.  All three then touch all banks once.  (With rows padded by
+// 16 and 32 bytes instead, conflicts took 40 % of the LDS's busy cycles.)
+template <int D> __device__ __forceinline__ int kv4_kswz(int row) { return D == 128 ? row & 15 : row >> 1 & 7; }
+template <int D> __device__ __forceinline__ int kv4_vswz(int row) { return 5 * (D == 128 ? row & 3 : row >> 1 & 1); }
+
 template <typename T, int D, int GH>
 __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
     const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
     const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ qsl, const int* __restrict__ seq_lens,
     const int* __restrict__ work_seq, const int* __restrict__ work_mblk, int nq, int nkv, int bs_log2, float scale_log2,
-    int num_blocks) {
+    int num_blocks, float* __restrict__ part_o, float* __restrict__ part_ml, int Z) {
   typedef typename Vec8<T>::type V8;
   constexpr int QB = KV4_BM / GH;                    // query rows of a workgroup
   constexpr int KS = D / 16, DT = D / 32, W = D / 32; // W: words of a thread's quarter row
-  constexpr int KST = D + 8, VST = D + 16;           // rows of the LDS tiles: a wave's 16-byte and transposing reads spread over the banks
-  __shared__ __attribute__((aligned(16))) T lds_k[2][KV4_BN * KST], lds_v[2][KV4_BN * VST];
+  constexpr int TILE = KV4_BN * D;
+  __shared__ __attribute__((aligned(16))) T lds_k[2][TILE], lds_v[2][TILE];
   const int seq = work_seq[blockIdx.x], mb = work_mblk[blockIdx.x];
   const int G = nq / nkv, h = blockIdx.y / (G / GH), head0 = h * G + blockIdx.y % (G / GH) * GH;
   const int q0 = qsl[seq], qlen = qsl[seq + 1] - q0;
   int L_in = seq_lens[seq];
   KGC_DCHECK_RANGE(L_in, 0, (bt_stride << bs_log2) + 1, "prefill seq_len");
   const int L = min(L_in, bt_stride << bs_log2), ctx0 = L - qlen;
-  const int qbase = mb * KV4_BM + blockIdx.z * QB;
+  const int qbase = mb * KV4_BM + blockIdx.z % GH * QB, slice = blockIdx.z / GH;
   if (qlen <= 0 || ctx0 < 0 || qbase >= qlen) return;  // the whole workgroup
   const int* bt = block_tables + (int64_t)seq * bt_stride;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, hi = lane >> 5;
   const int bs = 1 << bs_log2, bsm = bs - 1;
   const int64_t page_bytes = kv4_page_bytes(bs, D);
   const int wrow = qbase + wave / GH * 32, head = head0 + wave % GH;
-  const int tiles = (ctx0 + min(qbase + QB, qlen) - 1) / KV4_BN + 1;
+  const int all = (ctx0 + min(qbase + QB, qlen) - 1) / KV4_BN + 1;
+  const int first = (int)((int64_t)all * slice / Z), tiles = (int)((int64_t)all * (slice + 1) / Z);   // [first, tiles)
   // no row of this wave sees further (it may have none)
   const int wave_tiles = wrow < qlen ? (ctx0 + min(wrow + 32, qlen) - 1) / KV4_BN + 1 : 0;
 
@@ -74,14 +84,14 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
     const float a = kv4_scale(ks), b = kv4_scale(vs);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      *reinterpret_cast<u32x4*>(&lds_k[buf][tok * KST + part * (D / 4) + 8 * i]) = fp4x8_widen<T>(kw[i], a);
-      *reinterpret_cast<u32x4*>(&lds_v[buf][tok * VST + part * (D / 4) + 8 * i]) = fp4x8_widen<T>(vw[i], b);
+      *reinterpret_cast<u32x4*>(&lds_k[buf][tok * D + 8 * ((part * W + i) ^ kv4_kswz<D>(tok))]) = fp4x8_widen<T>(kw[i], a);
+      *reinterpret_cast<u32x4*>(&lds_v[buf][tok * D + 8 * ((part * W + i) ^ kv4_vswz<D>(tok))]) = fp4x8_widen<T>(vw[i], b);
     }
   };
 
-  int pg = page_of(0);
-  load(0, pg);
-  pg = page_of(min(1, tiles - 1));
+  int pg = page_of(first);                             // (an empty slice: a tile that is there, not used)
+  load(first, pg);
+  pg = page_of(first + 1);
   // q: lane (row col, hi) has elements 16 s + 8 hi .. + 7; rows behind the prompt's last one are that one again, not stored
   const int qi = min(wrow + col, qlen - 1), qpos = ctx0 + qi;
   V8 qf[KS];
@@ -96,17 +106,19 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
   }
   store(0);
   __syncthreads();
+  // this lane's part of a transposing read: row vr of four, 16-byte chunk vq of four
+  const int vr = (lane & 15) >> 2, vq = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
   f32x16 o[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
   float m = -INFINITY, l = 0.f;
-  for (int kt = 0; kt < tiles; ++kt) {
-    const int buf = kt & 1;
+  for (int kt = first; kt < tiles; ++kt) {
+    const int buf = (kt - first) & 1;
     if (kt + 1 < tiles) {
       load(kt + 1, pg);
-      pg = page_of(min(kt + 2, tiles - 1));
+      pg = page_of(kt + 2);
     }
     if (kt < wave_tiles) {
       const T* K = lds_k[buf];
@@ -119,7 +131,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
           Pack8<T> kf;
-          kf.u = *reinterpret_cast<const u32x4*>(K + (32 * g + col) * KST + 16 * j + 8 * hi);
+          kf.u = *reinterpret_cast<const u32x4*>(K + (32 * g + col) * D + 8 * ((2 * j + hi) ^ kv4_kswz<D>(col)));
           s[g] = mfma32x32x16(kf.v, qf[j], s[g]);
         }
       }
@@ -164,8 +176,8 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-          const T* src = V + (16 * j + 4 * hi + ((lane & 15) >> 2)) * VST + 32 * t + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-          const u32x2 a = ld_tr4(src), b = ld_tr4(src + 8 * VST);
+          const T* src = V + (16 * j + 4 * hi + vr) * D + 8 * ((4 * t + vq) ^ kv4_vswz<D>(vr)) + 4 * (lane & 1);
+          const u32x2 a = ld_tr4(src), b = ld_tr4(src + 8 * D);
           Pack8<T> vf;
           vf.u = u32x4{a.x, a.y, b.x, b.y};
           o[t] = mfma32x32x16(vf.v, pf[j], o[t]);
@@ -178,6 +190,20 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
   }
   if (wrow + col >= qlen) return;
   l += __shfl_xor(l, 32, 64);
+  if (Z > 1) {
+    const int64_t prow = ((int64_t)(q0 + qi) * nq + head) * Z + slice;
+    if (hi == 0) {
+      part_ml[2 * prow] = l != l ? INFINITY : m;         // a NaN is the merged row's too
+      part_ml[2 * prow + 1] = l;
+    }
+    float* dst = part_o + prow * D + 4 * hi;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4*>(dst + 32 * t + 8 * j) = f32x4{o[t][4 * j], o[t][4 * j + 1], o[t][4 * j + 2], o[t][4 * j + 3]};
+    return;
+  }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
   T* orow = out + ((int64_t)(q0 + qi) * nq + head) * D + 4 * hi;
 #pragma unroll
@@ -191,17 +217,52 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
     }
 }
 
+// A wave per row of the work items' blocks and heads: lane z has slice z's maximum and sum.
+constexpr int KV4_MAX_SLICES = 32;
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(
+    T* __restrict__ out, const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ qsl,
+    const int* __restrict__ seq_lens, const int* __restrict__ work_seq, const int* __restrict__ work_mblk, int nq, int cap,
+    int Z) {
+  const int seq = work_seq[blockIdx.x], q0 = qsl[seq], qlen = qsl[seq + 1] - q0;
+  const int lane = threadIdx.x & 63, r = work_mblk[blockIdx.x] * KV4_BM + blockIdx.z * 4 + (threadIdx.x >> 6);
+  if (r >= qlen || min(seq_lens[seq], cap) < qlen) return;    // as the kernel above
+  const int64_t row = (int64_t)(q0 + r) * nq + blockIdx.y;
+  const float m = lane < Z ? part_ml[2 * (row * Z + lane)] : -INFINITY;
+  const float l = lane < Z ? part_ml[2 * (row * Z + lane) + 1] : 0.f;
+  const float top = wave_max(m), w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+  const float total = wave_sum(w == 0.f ? 0.f : w * l);
+  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  constexpr int E = D / 64;
+  float acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int z = 0; z < Z; ++z) {
+    const float f = __shfl(w, z, 64);
+    if (f == 0.f) continue;                                  // nothing seen there, or nothing that counts
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += f * part_o[(row * Z + z) * D + lane * E + e];
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) out[row * D + lane * E + e] = from_f<T>(acc[e] * inv);
+}
+
 template <typename T, int D>
 static void kv4_prefill_dispatch(const Kv4Prefill& a, float sl2, hipStream_t s) {
   const int G = a.nq / a.nkv;
 #define KGC_KV4_PF(GH)                                                                                                \
-  kv4_prefill_kernel<T, D, GH><<<dim3(a.n_work, a.nkv * (G / GH), GH), 256, 0, s>>>(                                     \
+  kv4_prefill_kernel<T, D, GH><<<dim3(a.n_work, a.nkv * (G / GH), GH * a.Z), 256, 0, s>>>(                                     \
       (const T*)a.q, (T*)a.out, (const uint8_t*)a.k_cache, (const uint8_t*)a.v_cache, a.block_tables, a.bt_stride,      \
-      a.query_start_loc, a.seq_lens, a.work_seq, a.work_mblk, a.nq, a.nkv, a.bs_log2, sl2, a.num_blocks)
+      a.query_start_loc, a.seq_lens, a.work_seq, a.work_mblk, a.nq, a.nkv, a.bs_log2, sl2, a.num_blocks,        \
+      a.part_o, a.part_ml, a.Z)
   if (G % 4 == 0) KGC_KV4_PF(4);
   else if (G % 2 == 0) KGC_KV4_PF(2);
   else KGC_KV4_PF(1);
 #undef KGC_KV4_PF
+  if (a.Z > 1)
+    kv4_prefill_merge_kernel<T, D><<<dim3(a.n_work, a.nq, KV4_BM / 4), 256, 0, s>>>(
+        (T*)a.out, a.part_o, a.part_ml, a.query_start_loc, a.seq_lens, a.work_seq, a.work_mblk, a.nq,
+        a.bt_stride << a.bs_log2, a.Z);
 }
 
 void launch_kv4_prefill(int dtype, const Kv4Prefill& a, float scale, hipStream_t s) {

@@ -109,6 +109,8 @@ struct Kv4Prefill {
   void* out;
   const int *block_tables, *query_start_loc, *seq_lens, *work_seq, *work_mblk;
   int bt_stride, n_work, nq, nkv, D, bs_log2, num_blocks;
+  float *part_o, *part_ml;   // Z > 1: [rows, nq, Z, D] and [rows, nq, Z, 2]
+  int Z;                     // workgroups that share an item's keys, 1 to 32
 };
 void launch_kv4_prefill(int dtype, const Kv4Prefill& a, float scale, hipStream_t s);
 // debug builds: sticky bounds-check error words of the K1 / K2 / K3 translation units

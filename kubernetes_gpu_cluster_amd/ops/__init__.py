@@ -250,6 +250,11 @@ def _decode_z_cap(ws, B: int, nq: int) -> int:
 KV4_TARGET_WAVES = 2048      # 4-bit decode: 8 resident waves per CU
 
 
+def kv4_decode_waves(pairs: int) -> int:
+    """Waves that share a slice (csrc/kernels/kv4_decode.hip kv4_decode_waves)."""
+    return 1 if pairs >= 1024 else 4 if pairs >= 512 else 8 if pairs >= 64 else 4
+
+
 def decode_grid_z(batch: int, num_kv_heads: int, max_ctx: int, target_waves: int = 0,
                   capacity: bool = False, cache_dtype: Optional[torch.dtype] = None) -> int:
     """z-slices of the decode grid: enough waves to fill 256 CUs, bounded by the
@@ -265,11 +270,16 @@ def decode_grid_z(batch: int, num_kv_heads: int, max_ctx: int, target_waves: int
     ``capacity``: max_ctx is what the rows may come to (a captured graph).  Empty slices cost too, so that the 4-wave
     kernel has no more there than are as fast for short rows: 56 pairs, 32 slices instead of the 19 of 8192 tokens, 40, 500
     tokens 11.9 -> 13.5, 15.0 -> 17.5; 8 instead of 3 of 544 8.8 -> 9.5, 15.5 -> 12.5 (4: 8.8, 11.7).
-    ``cache_dtype`` uint8: the 4-bit cache, whose kernel is one wave per slice at any size."""
+    ``cache_dtype`` uint8: the 4-bit cache, a slice of which has two chunks or more for each of its
+    waves; its merge takes up to 64 slices in one round trip (csrc/kernels/kv4_decode.hip)."""
     pairs = max(1, batch * num_kv_heads)
     if cache_dtype == torch.uint8:
         chunks = max(1, math.ceil(max_ctx / DECODE_CHUNK))
-        return max(1, min(math.ceil((target_waves or KV4_TARGET_WAVES) / pairs), math.ceil(chunks / 2), 1024))
+        waves = kv4_decode_waves(pairs)
+        if chunks <= (64 if pairs >= 64 else 16):
+            return 1
+        return max(1, min(math.ceil((target_waves or KV4_TARGET_WAVES) / (pairs * waves)),
+                          math.ceil(chunks / (2 * waves)), 64))
     if decode_uses_wave(batch, num_kv_heads):
         chunks = max(1, math.ceil(max_ctx / DECODE_CHUNK))
         if not target_waves and chunks <= (10 if pairs >= DECODE_LONG_PAIRS else 4):
@@ -373,6 +383,17 @@ def prefill_work_list(query_lens: list[int], seq_lens: list[int]) -> tuple[list[
     return [i for _, i, _ in items], [m for _, _, m in items]
 
 
+def kv4_prefill_slices(rows: int, items: int, seqs: int, num_heads: int, num_kv_heads: int, max_len: int) -> int:
+    """Workgroups that share the keys of each item of a prompt step over a 4-bit cache (csrc/kernels/kv4_prefill.hip): as
+    many as fill the CUs twice, each with 4 tiles of 64 keys or more."""
+    if os.environ.get("KV4_PZ"):
+        return int(os.environ["KV4_PZ"])
+    g = num_heads // num_kv_heads
+    heads = 4 if g % 4 == 0 else 2 if g % 2 == 0 else 1
+    blocks = min(items * heads, rows * heads // PREFILL_BLOCK_M + seqs) * (num_heads // heads)
+    return max(1, min(512 // max(blocks, 1), math.ceil(max_len / 64) // 4, 32))
+
+
 def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                       block_tables: torch.Tensor, query_start_loc: torch.Tensor,
                       seq_lens: torch.Tensor, scale: float, work_seq: torch.Tensor = None,
@@ -392,8 +413,14 @@ def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         work_mblk = torch.tensor(wm, dtype=torch.int32, device=q.device)
     if out is None:
         out = torch.empty_like(q)
+    partials = None
+    if k_cache.dtype == torch.uint8:
+        z = kv4_prefill_slices(q.shape[0], work_seq.shape[0], block_tables.shape[0], q.shape[1], k_cache.shape[1],
+                               max_len or block_tables.shape[1] * k_cache.shape[2])
+        if z > 1:
+            partials = torch.empty(z * q.numel() // q.shape[2] * (q.shape[2] + 2), dtype=torch.float32, device=q.device)
     _k().prefill_attention(out, q, k_cache, v_cache, block_tables, query_start_loc, seq_lens,
-                           work_seq, work_mblk, scale, k_scale, v_scale, max_len)
+                           work_seq, work_mblk, scale, k_scale, v_scale, max_len, partials)
     return out
 
 

@@ -198,6 +198,9 @@ DECODE = [
     (8, 8, 128, 16, [1500]),
     (10, 2, 64, 32, [500, 31, 96]),
     (7, 1, 128, 128, [257, 128]),
+    (8, 8, 64, 32, [2100, 1, 0, 90, 64, 33, 500, 2, 7]),
+    (8, 8, 64, 16, [1 + 7 * i % 67 for i in range(70)]),
+    (8, 8, 64, 32, [3 * i % 71 for i in range(130)]),
 ]
 
 
@@ -255,6 +258,46 @@ def test_prompts(gpu, dt, nq, nkv, d, bs, new, old):
                                 torch.tensor(totals, dtype=torch.int32, device=gpu), d ** -0.5, out=out)
     assert got.data_ptr() == out.data_ptr() and (out[-3:] == 7).all()
     _check_attention(got[:-3].cpu(), q, kc, vc, bt, new, totals, d ** -0.5)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("nq,nkv,d,bs,new,old", [
+    (4, 1, 128, 32, [33, 1, 130], [1900, 700, 0]),
+    (3, 3, 64, 16, [40, 5], [0, 1000]),
+    (16, 2, 128, 64, [7], [1500]),
+])
+@pytest.mark.parametrize("z", [2, 5, 32])
+def test_prompts_in_slices(gpu, dt, nq, nkv, d, bs, new, old, z):
+    """z workgroups per item, among them some that see nothing; the merge leaves other rows as they were."""
+    q, kc, vc, bt, totals = _attention_case(z + sum(new), nq, nkv, d, bs, dt, new, old)
+    qg = torch.cat([q, torch.zeros(3, nq, d, dtype=dt)]).to(gpu)
+    ws, wm = (torch.tensor(w, dtype=torch.int32, device=gpu) for w in ops.prefill_work_list(new, totals))
+    parts = torch.full((z * len(qg) * nq * (d + 2),), float("nan"), device=gpu)
+    out = torch.full_like(qg, 7)
+    torch.ops.kgc.prefill_attention(out, qg, kc.to(gpu), vc.to(gpu), bt.to(gpu), _starts(new).to(gpu),
+                                    torch.tensor(totals, dtype=torch.int32, device=gpu), ws, wm, d ** -0.5, 1.0, 1.0, 0,
+                                    parts)
+    assert (out[-3:] == 7).all()
+    _check_attention(out[:-3].cpu(), q, kc, vc, bt, new, totals, d ** -0.5)
+
+
+@pytest.mark.parametrize("z", [1, 3])
+def test_nan_queries_stay_with_their_rows(gpu, z):
+    """A NaN or infinite query row is NaN, with slices too, and no other row is."""
+    new, old = [70, 3], [600, 900]
+    q, kc, vc, bt, totals = _attention_case(2, 4, 2, 64, 32, torch.bfloat16, new, old)
+    q[5, 1], q[71, 2, 7] = float("nan"), float("inf")
+    n = torch.tensor(totals, dtype=torch.int32, device=gpu)
+    ws, wm = (torch.tensor(w, dtype=torch.int32, device=gpu) for w in ops.prefill_work_list(new, totals))
+    parts = torch.empty(z * q.numel() // 64 * 66, device=gpu) if z > 1 else None
+    out = torch.empty_like(q).to(gpu)
+    torch.ops.kgc.prefill_attention(out, q.to(gpu), kc.to(gpu), vc.to(gpu), bt.to(gpu), _starts(new).to(gpu), n, ws, wm,
+                                    0.125, 1.0, 1.0, 0, parts)
+    bad = torch.zeros(73, 4, dtype=torch.bool)
+    bad[5, 1] = bad[71, 2] = True
+    assert torch.equal(out.cpu().isnan().all(-1), bad) and torch.equal(out.cpu().isnan().any(-1), bad)
+    dec = ops.paged_attention_decode(q[4:6].contiguous().to(gpu), kc.to(gpu), vc.to(gpu), bt.to(gpu), n, 0.125, None, z)
+    assert torch.equal(dec.cpu().isnan().all(-1), bad[4:6]) and torch.equal(dec.cpu().isnan().any(-1), bad[4:6])
 
 
 @pytest.mark.parametrize("dt", DT)
@@ -410,6 +453,11 @@ def test_refusals(gpu):
     no("query_start_loc", pre, q, kc, kc, bt[:1], n, n[:1], 1.0, n, n)
     no("seq_lens", pre, q, kc, kc, bt[:2], n, n[:1], 1.0, n, n)
     no("work list", pre, q, kc, kc, bt[:2], n, n[:2], 1.0, n, n[:2])
+    no("slices", torch.ops.kgc.prefill_attention, q, q, kc, kc, bt[:1], n[:2], n[:1], n[:1], n[:1], 1.0, 1.0, 1.0, 0,
+       torch.zeros(12 * 129, device=gpu))
+    wide = (torch.zeros(4, 2, 16, d, dtype=bf, device=gpu), torch.zeros(4, 2, 2, d, 8, dtype=bf, device=gpu))
+    no("4-bit", torch.ops.kgc.prefill_attention, q, q, *wide, bt[:1], n[:2], n[:1], n[:1], n[:1], 1.0, 1.0, 1.0, 0,
+       torch.zeros(12 * 130, device=gpu))
     no("head_dim", wr, x, pos, torch.zeros(8, 96, device=gpu), kc, kc, pos, 4, 2, 96)
     no("positions", wr, x, pos[:2], table, kc, kc, pos, 4, 2, d)
     no("slot_mapping", wr, x, pos, table, kc, kc, pos[:2], 4, 2, d)
