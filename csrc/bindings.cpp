@@ -194,20 +194,22 @@ void kv4_write(const Tensor& qkv, int64_t stride, int64_t S, int64_t slice_strid
   kgc::launch_kv4_write(dt_code(q_out), w, ax, stream());
 }
 
-void kv4_read(Tensor out, Tensor cache, Tensor slots) {
+// -> [n, nkv, d]
+Tensor kv4_read(Tensor cache, Tensor slots, at::ScalarType dtype) {
   check_gpu(cache, "cache");
   c10::hip::HIPGuardMasqueradingAsCUDA g(cache.device());
-  TORCH_CHECK(out.dim() == 3 && out.is_contiguous() &&
-              (out.scalar_type() == at::kBFloat16 || out.scalar_type() == at::kHalf),
-              "kgc.kv4_read: out bf16 / fp16 [n, nkv, d] contiguous");
-  check_kv4(cache, cache, out.size(1), out.size(2), out);
-  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.numel() == out.size(0),
-              "kgc.kv4_read: slots int64 [n]");
-  check_same_dev(out, slots, "slots");
-  aligned16(out, "out");
-  TORCH_CHECK(out.numel() / 8 < ((int64_t)1 << 31) * 256, "kgc.kv4_read: rows");
-  kgc::launch_kv4_read(dt_code(out), out.data_ptr(), cache.data_ptr(), slots.data_ptr<int64_t>(), out.size(0),
-                       (int)out.size(1), (int)out.size(2), (int)cache.size(2), (int)cache.size(0), stream());
+  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, "kgc.kv4_read: bf16 / fp16 values");
+  TORCH_CHECK(cache.dim() == 4, "4-bit cache: uint8 [nb, nkv, bs, d / 2 + d / 32]");
+  const int64_t nkv = cache.size(1), d = cache.size(3) * 32 / 17;
+  check_kv4(cache, cache, nkv, d, cache);
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous(), "kgc.kv4_read: slots int64 [n]");
+  check_same_dev(cache, slots, "slots");
+  TORCH_CHECK(slots.numel() * nkv * (d / 8) < ((int64_t)1 << 31) * 256, "kgc.kv4_read: rows");
+  Tensor out = at::empty({slots.numel(), nkv, d}, cache.options().dtype(dtype));
+  if (cache.size(0) == 0) out.zero_();
+  kgc::launch_kv4_read(dt_code(out), out.data_ptr(), cache.data_ptr(), slots.data_ptr<int64_t>(), out.size(0), (int)nkv,
+                       (int)d, (int)cache.size(2), (int)cache.size(0), stream());
+  return out;
 }
 
 // what both attention forms over a 4-bit cache ask for
@@ -2996,7 +2998,7 @@ TORCH_LIBRARY(kgc, m) {
         "Tensor(b!) k_cache, Tensor(c!) v_cache, Tensor slot_mapping, Tensor? q_norm_w, "
         "Tensor? k_norm_w, int nq, int nkv, int d, float eps, bool use_rope, float k_scale=1.0, "
         "float v_scale=1.0, int[]? sections=None) -> ()");
-  m.def("kv4_read(Tensor(a!) out, Tensor cache, Tensor slots) -> ()");
+  m.def("kv4_read(Tensor cache, Tensor slots, ScalarType dtype) -> Tensor");
   m.def("paged_decode(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, "
         "Tensor block_tables, Tensor ctx_lens, Tensor(b!) max_logits, Tensor(c!) exp_sums, "
         "Tensor(d!) tmp_out, int Z, float scale, float k_scale=1.0, "

@@ -4,7 +4,8 @@
 // wider caches: optional per-head RMS norm, NeoX rotation by one position or by one per axis, q stored in T, k and v as
 // e2m1 numbers with their scales.  A thread has the 16-byte chunk pair (c, c + d / 2) of HG heads that lie side by side in the
 // row: the pair is what the rotation needs, four neighbouring lanes hold a block of 32, and cos / sin are loaded once
-// for the heads.
+// for the heads.  A wave has the same heads of 8 tokens (16 with heads of 64), so that its lanes take the same way and a page's
+// rows are written side by side.
 //
 // k is rotated in 64 bits, where the products are exact and the sum is rounded once, and then to the nearest code: a key
 // next to the border of two codes, which are up to a third apart, then has the code that the mathematics gives it, whatever order of
@@ -25,11 +26,12 @@ __global__ __launch_bounds__(KV4_NT) void kv4_write_kernel(
     const int64_t* __restrict__ slot_mapping, const T* __restrict__ qn_w, const T* __restrict__ kn_w, int64_t T_, int nq,
     int nkv, int d, int bs, float eps, int num_blocks, RopeAxes ax) {
   const int tph = d >> 4, half = d >> 1;               // threads per head: 4 or 8, whole lane groups
-  const int heads = nq + 2 * nkv, groups = (heads + HG - 1) / HG, per = groups * tph;
-  const int64_t item = (int64_t)blockIdx.x * KV4_NT + threadIdx.x;
-  if (item >= T_ * per) return;                        // whole lane groups
-  const int64_t t = item / per;
-  const int r = (int)(item - t * per), h0 = r / tph * HG, c = r % tph;
+  const int heads = nq + 2 * nkv, groups = (heads + HG - 1) / HG, tpw = 64 / tph;
+  const int64_t wave = (int64_t)blockIdx.x * (KV4_NT / 64) + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, c = lane % tph;
+  const int64_t t = wave / groups * tpw + lane / tph;
+  if (t >= T_) return;                                 // whole lane groups
+  const int h0 = (int)(wave % groups) * HG;
   const int64_t row = t * qkv_stride;
   int64_t slot = slot_mapping[t];
   KGC_DCHECK_RANGE(slot, -1, (int64_t)num_blocks * bs, "KV slot");
@@ -163,26 +165,39 @@ __global__ __launch_bounds__(KV4_NT) void kv4_write_kernel(
   }
 }
 
-// Rows of the cache as the values they stand for; slots outside the pool give zeros.  8 elements a thread.
-template <typename T>
+// Rows of the cache as the values they stand for; slots outside the pool give zeros.  8 elements a thread, U times.
+template <typename T, int U>
 __global__ __launch_bounds__(KV4_NT) void kv4_read_kernel(T* __restrict__ out, const uint8_t* __restrict__ cache,
                                                           const int64_t* __restrict__ slots, int64_t n, int nkv, int d,
                                                           int bs, int num_blocks) {
   const int per = nkv * (d >> 3);
-  const int64_t item = (int64_t)blockIdx.x * KV4_NT + threadIdx.x;
-  if (item >= n * per) return;
-  const int64_t i = item / per;
-  const int r = (int)(item - i * per), h = r / (d >> 3), c = r % (d >> 3);
-  const int64_t slot = slots[i];
-  u32x4 v = {0u, 0u, 0u, 0u};
-  if (slot >= 0 && slot < (int64_t)num_blocks * bs) {
-    const int64_t blk = slot / bs;
-    const int off = (int)(slot - blk * bs);
-    const uint8_t* page = cache + (blk * nkv + h) * kv4_page_bytes(bs, d);
-    v = fp4x8_widen<T>(reinterpret_cast<const uint32_t*>(page + off * (d >> 1))[c],
-                       kv4_scale(page[bs * (d >> 1) + off * (d >> 5) + (c >> 2)]));
+  const int64_t first = (int64_t)blockIdx.x * (KV4_NT * U) + threadIdx.x;
+  int64_t at[U];
+  int off[U], c[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t i = min(first + u * KV4_NT, n * per - 1) / per;
+    at[u] = slots[i];
   }
-  reinterpret_cast<u32x4*>(out)[item] = v;
+  uint32_t w[U];
+  uint8_t s[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t item = min(first + u * KV4_NT, n * per - 1);
+    const int r = (int)(item % per), h = r / (d >> 3);
+    c[u] = r % (d >> 3);
+    const bool there = at[u] >= 0 && at[u] < (int64_t)num_blocks * bs;
+    if (!there) at[u] = 0;                             // (a pool without pages has no slots: nothing is launched)
+    const int64_t blk = at[u] / bs;
+    off[u] = (int)(at[u] - blk * bs);
+    const uint8_t* page = cache + (blk * nkv + h) * kv4_page_bytes(bs, d);
+    w[u] = reinterpret_cast<const uint32_t*>(page + off[u] * (d >> 1))[c[u]];
+    s[u] = page[bs * (d >> 1) + off[u] * (d >> 5) + (c[u] >> 2)];
+    if (!there) w[u] = 0, s[u] = 127;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (first + u * KV4_NT < n * per) reinterpret_cast<u32x4*>(out)[first + u * KV4_NT] = fp4x8_widen<T>(w[u], kv4_scale(s[u]));
 }
 
 template <typename T, bool SL, bool AXES, int HG>
@@ -207,10 +222,17 @@ static void kv4_write_norm(const Kv4Write& w, const RopeAxes& ax, int64_t blocks
 
 template <typename T>
 static void kv4_write_dispatch(const Kv4Write& w, const RopeAxes& ax, hipStream_t s) {
-  auto blocks = [&](int hg) { return (w.T * ((w.nq + 2 * w.nkv + hg - 1) / hg) * (w.d >> 4) + KV4_NT - 1) / KV4_NT; };
+  const int64_t tokens = (w.T * (w.d >> 4) + 63) / 64;           // in waves' worth
+  auto blocks = [&](int hg) { return (tokens * ((w.nq + 2 * w.nkv + hg - 1) / hg) + KV4_NT / 64 - 1) / (KV4_NT / 64); };
   if (w.S > 0) {
     if (ax.n) kv4_write_norm<T, true, true, 1>(w, ax, blocks(1), s);
     else kv4_write_norm<T, true, false, 1>(w, ax, blocks(1), s);
+  } else if (blocks(1) <= 4096) {
+    // Few workgroups: a head per thread, all loads of a call on their way at once; many: cos / sin for four.  us with both
+    // caches' rows read back, one head -> four: 256 rows of 32 / 8 heads 9.4 -> 12.1, 1000 12.8 -> 15.0, 2000 20.0 -> 19.6, 16384
+    // 100.5 -> 97.6 (the write alone 75, 353 MB); 4000 of 12 / 12 heads of 64 18.0 -> 21.0.
+    if (ax.n) kv4_write_norm<T, false, true, 1>(w, ax, blocks(1), s);
+    else kv4_write_norm<T, false, false, 1>(w, ax, blocks(1), s);
   } else if (ax.n) {
     kv4_write_norm<T, false, true, 4>(w, ax, blocks(4), s);
   } else {
@@ -224,14 +246,23 @@ void launch_kv4_write(int dtype, const Kv4Write& w, const RopeAxes& ax, hipStrea
   else kv4_write_dispatch<f16>(w, ax, s);
 }
 
+template <typename T>
+static void kv4_read_dispatch(void* out, const void* cache, const int64_t* slots, int64_t n, int nkv, int d, int bs,
+                              int num_blocks, hipStream_t s) {
+  const int64_t items = n * nkv * (d >> 3);
+  if (items < (1 << 20))
+    kv4_read_kernel<T, 1><<<(unsigned)((items + KV4_NT - 1) / KV4_NT), KV4_NT, 0, s>>>(
+        (T*)out, (const uint8_t*)cache, slots, n, nkv, d, bs, num_blocks);
+  else
+    kv4_read_kernel<T, 4><<<(unsigned)((items + 4 * KV4_NT - 1) / (4 * KV4_NT)), KV4_NT, 0, s>>>(
+        (T*)out, (const uint8_t*)cache, slots, n, nkv, d, bs, num_blocks);
+}
+
 void launch_kv4_read(int dtype, void* out, const void* cache, const int64_t* slots, int64_t n, int nkv, int d, int bs,
                      int num_blocks, hipStream_t s) {
-  if (n == 0) return;
-  const unsigned blocks = (unsigned)((n * nkv * (d >> 3) + KV4_NT - 1) / KV4_NT);
-  if (dtype == DT_BF16)
-    kv4_read_kernel<<<blocks, KV4_NT, 0, s>>>((bf16*)out, (const uint8_t*)cache, slots, n, nkv, d, bs, num_blocks);
-  else
-    kv4_read_kernel<<<blocks, KV4_NT, 0, s>>>((f16*)out, (const uint8_t*)cache, slots, n, nkv, d, bs, num_blocks);
+  if (n == 0 || num_blocks == 0) return;
+  if (dtype == DT_BF16) kv4_read_dispatch<bf16>(out, cache, slots, n, nkv, d, bs, num_blocks, s);
+  else kv4_read_dispatch<f16>(out, cache, slots, n, nkv, d, bs, num_blocks, s);
 }
 
 KGC_DEBUG_TU(kv4_cache)

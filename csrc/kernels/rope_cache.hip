@@ -224,13 +224,14 @@ __global__ __launch_bounds__(ROPE_NT) void rope_kv_kernel(
 // rows, 8 heads of 128, 134 MB: 75 us, 28 here, the rate of a large copy; fp8 cache, which had the
 // per-token kernel, 86 -> 22).  Up to 1000 rows that do lie with the groups take 4.7 us where blocks
 // of the step's rows took 4.0: a thread has four pairs or eight rows.
+// AXES: as everywhere, cos / sin of a chunk's own axis.
 constexpr int KVG_NT = 256;
-template <typename T, bool KV8>
+template <typename T, bool KV8, bool AXES>
 __global__ __launch_bounds__(KVG_NT) void kv_group_kernel(
     const T* __restrict__ qkv, int64_t qkv_stride, const int64_t* __restrict__ positions,
     const float* __restrict__ cos_sin, void* __restrict__ k_cache, void* __restrict__ v_cache,
     const int64_t* __restrict__ slot_mapping, int T_, int nq, int nkv, int d, int bs, int bs_shift,
-    int num_blocks, float k_inv, float v_inv, int groups) {
+    int num_blocks, float k_inv, float v_inv, int groups, RopeAxes ax) {
   typedef std::conditional_t<KV8, uint8_t, T> C;
   C* kc = reinterpret_cast<C*>(k_cache);
   C* vc = reinterpret_cast<C*>(v_cache);
@@ -246,7 +247,7 @@ __global__ __launch_bounds__(KVG_NT) void kv_group_kernel(
     int64_t sl = slot_mapping[row];
     KGC_DCHECK_RANGE(sl, -1, (int64_t)num_blocks * bs, "KV slot");
     slot = sl < 0 ? -1 : (int)sl;
-    if (slot >= 0) pos = (int)positions[row];
+    if (!AXES && slot >= 0) pos = (int)positions[row];
   }
   const int up = __shfl_down(slot, 1, 64);
   const uint32_t next = (uint32_t)__ballot(slot >= 0 && up == slot + 1 && lane < 21);
@@ -282,12 +283,19 @@ __global__ __launch_bounds__(KVG_NT) void kv_group_kernel(
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float* cs = cos_sin + (int64_t)ps[i] * d + c * 8;
-        const float4 c0 = *reinterpret_cast<const float4*>(cs), c1 = *reinterpret_cast<const float4*>(cs + 4);
-        const float4 s0 = *reinterpret_cast<const float4*>(cs + half);
-        const float4 s1 = *reinterpret_cast<const float4*>(cs + half + 4);
-        const float co[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-        const float si[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+        float co[8], si[8];
+        if constexpr (AXES) {
+          axes_cos_sin(ax, positions, min(t0 + par + 2 * i, T_ - 1), cos_sin, d, c * 8, co, si);
+        } else {
+          const float* cs = cos_sin + (int64_t)ps[i] * d + c * 8;
+          const float4 c0 = *reinterpret_cast<const float4*>(cs), c1 = *reinterpret_cast<const float4*>(cs + 4);
+          const float4 s0 = *reinterpret_cast<const float4*>(cs + half);
+          const float4 s1 = *reinterpret_cast<const float4*>(cs + half + 4);
+          co[0] = c0.x; co[1] = c0.y; co[2] = c0.z; co[3] = c0.w;
+          co[4] = c1.x; co[5] = c1.y; co[6] = c1.z; co[7] = c1.w;
+          si[0] = s0.x; si[1] = s0.y; si[2] = s0.z; si[3] = s0.w;
+          si[4] = s1.x; si[5] = s1.y; si[6] = s1.z; si[7] = s1.w;
+        }
         Pack8<T> oa, ob;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -391,19 +399,44 @@ static void rope_dispatch(const void* qkv, int64_t qkv_stride, int S, int64_t ss
       (const T*)kn, nq, nkv, d, bs, eps, k_inv, v_inv, num_blocks, ax)
 #define KGC_ROPE_LAUNCH(N, R, O) KGC_ROPE_LAUNCH_AXES(N, R, O, false)
   const bool norm = qn != nullptr;
+  auto kv_groups = [&] { return (d & 15) == 0 && (bs & 7) == 0 && (int64_t)num_blocks * bs < INT_MAX; };
+  const int units = nkv * (d >> 2), groups = units <= 64 ? 4 : units <= 128 ? 2 : 1;      // of one 8-row group
   if (ax.n) {                   // (the host: rotated, q asked for)
+    if constexpr (!SL) {
+      // Two launches, q by rows and k / v by 8-row groups, from 4M elements on; us, 32 / 8 heads of 128 in 16-bit pages, one launch ->
+      // two: 500 rows 10.1 -> 11.0, 1000 13.0 -> 12.2, 2000 22.0 -> 17.2, 12000 106.7 -> 72.5; 8 / 1 heads 1000 7.1 -> 8.9,
+      // 4000 14.6 -> 12.6; 1000 of 12 / 12 heads of 64 12.0 -> 12.3.
+      if (!norm && kv_groups() && (d == 64 || d == 128) && (int64_t)T_ * (nq + 2 * nkv) * d >= 4 << 20 &&
+          reinterpret_cast<uintptr_t>(qkv) % 16 == 0 && reinterpret_cast<uintptr_t>(q_out) % 16 == 0) {
+        Kv4Write w{};           // q alone: no kv heads
+        w.qkv = qkv;
+        w.qkv_stride = qkv_stride;
+        w.positions = pos;
+        w.cos_sin = cs;
+        w.q_out = q_out;
+        w.slots = slots;
+        w.T = T_;
+        w.nq = nq;
+        w.d = d;
+        w.bs = bs;
+        w.num_blocks = num_blocks;
+        w.use_rope = true;
+        launch_kv4_write(std::is_same_v<T, bf16> ? DT_BF16 : DT_F16, w, ax, s);
+        kv_group_kernel<T, KV8, true><<<(T_ + 8 * groups - 1) / (8 * groups), KVG_NT, 0, s>>>(
+            (const T*)qkv, qkv_stride, pos, cs, kc, vc, slots, T_, nq, nkv, d, bs,
+            (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1, num_blocks, k_inv, v_inv, groups, ax);
+        return;
+      }
+    }
     if (norm) KGC_ROPE_LAUNCH_AXES(true, true, false, true);
     else KGC_ROPE_LAUNCH_AXES(false, true, false, true);
     return;
   }
   if constexpr (!SL) {
-    const int64_t slots_end = (int64_t)num_blocks * bs;
-    if (kvo && rope && !norm && rope_kvg() && (d & 15) == 0 && (bs & 7) == 0 && slots_end < INT_MAX) {
-      const int units = nkv * (d >> 2);      // of one 8-row group
-      const int groups = units <= 64 ? 4 : units <= 128 ? 2 : 1;
-      kv_group_kernel<T, KV8><<<(T_ + 8 * groups - 1) / (8 * groups), KVG_NT, 0, s>>>(
+    if (kvo && rope && !norm && rope_kvg() && kv_groups()) {
+      kv_group_kernel<T, KV8, false><<<(T_ + 8 * groups - 1) / (8 * groups), KVG_NT, 0, s>>>(
           (const T*)qkv, qkv_stride, pos, cs, kc, vc, slots, T_, nq, nkv, d, bs,
-          (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1, num_blocks, k_inv, v_inv, groups);
+          (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1, num_blocks, k_inv, v_inv, groups, ax);
       return;
     }
   }

@@ -177,9 +177,7 @@ def kv4_read(cache: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype) -> to
     them is a number of the ``dtype`` it was written from); slots outside the pool give zeros."""
     if not _gpu(cache):
         return ref.kv4_read(cache, slots, dtype)
-    out = torch.empty(slots.shape[0], cache.shape[1], ref.kv4_head_dim(cache), dtype=dtype, device=cache.device)
-    _k().kv4_read(out, cache, slots)
-    return out
+    return _k().kv4_read(cache, slots, dtype)
 
 
 def kv_write_rope(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,

@@ -26,7 +26,7 @@ def _check_rows(got, want, u, size):
 @pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("nq,nkv,d,bs", [(32, 8, 128, 32), (5, 1, 64, 16), (3, 3, 128, 64), (12, 12, 64, 32)])
 @pytest.mark.parametrize("T,sections,slices", [(1, None, 0), (133, None, 0), (133, (10, 9, -1), 0), (37, None, 3),
-                                               (37, (8, 8, 8, -1), 2), (300, (-1,), 0)])
+                                               (37, (8, 8, 8, -1), 2), (300, (-1,), 0), (1500, (9, -1), 0)])
 def test_write(gpu, dt, nq, nkv, d, bs, T, sections, slices):
     g = _gen(T + d)
     if sections:
@@ -131,16 +131,23 @@ def test_write_with_norms(gpu, cache, sections):
 
 @pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("cache", ["auto", "fp8"])
-@pytest.mark.parametrize("T,sections,slices", [(77, (16, 24, 24), 0), (77, (5, 0, 40, 19), 0), (9, (64,), 2)])
+@pytest.mark.parametrize("T,sections,slices", [(77, (16, 24, 24), 0), (77, (5, 0, 40, 19), 0), (9, (64,), 2), (700, (16, 24, 24), 0),
+                                               (521, (60, 1, 3), 0)])
 def test_axes_of_the_wider_caches(gpu, dt, cache, T, sections, slices):
     g, nq, nkv, d, bs = _gen(7), 8, 2, 128, 16
     t = torch.float8_e4m3fn if cache == "fp8" else dt
-    mk = lambda: (torch.zeros(8, nkv, bs, d).to(t).to(gpu), torch.zeros(8, nkv, bs // 8, d, 8).to(t).to(gpu))   # noqa: E731
+    nb = max(8, T // 16 + 3)
+    mk = lambda: (torch.zeros(nb, nkv, bs, d).to(t).to(gpu), torch.zeros(nb, nkv, bs // 8, d, 8).to(t).to(gpu))   # noqa: E731
     x = torch.randn(max(slices, 1), T, (nq + 2 * nkv) * d, generator=g)
     x = x.to(gpu) if slices else x[0].to(dt).to(gpu)
     table = ref.rope_cos_sin_cache(d, 90, 10000.0)
     pos = torch.randint(-5, 99, (len(sections), T), generator=g)
-    slots = torch.randperm(8 * bs, generator=g)[:T].to(gpu)
+    slots = torch.randperm(nb * bs, generator=g)[:T]
+    if T > 100:                                               # runs that start in an 8-key group, and padding
+        slots = (torch.arange(T) + 5) % (nb * bs)
+        slots[100:] += 3
+        slots[-3:] = -1
+    slots = slots.to(gpu)
     kc, vc = mk()
     q = ops.rope_kv_write(x, pos.to(gpu), table.to(gpu), kc, vc, slots, nq, nkv, d, dtype=dt, sections=sections)
     # each pair as the one-position kernel turns it, from a table of that axis's rows
@@ -471,5 +478,6 @@ def test_refusals(gpu):
     no("empty cos_sin", wr, x, p2, table[:0], kc, kc, pos, 4, 2, d, sections=(32, 32))
     no("write q too", ops.kv_write_rope, x, pos, table, kc, kc, pos, 4, 2, d)
     no("4-D / v_cache 5-D", ops.prefill_attention_rope, x, table, kc, kc, bt[:1], n[:2], n[:1], 1.0, 4, d, n[:1], n[:1])
-    no("slots int64", torch.ops.kgc.kv4_read, torch.zeros(3, 2, d, dtype=bf, device=gpu), kc, pos.int())
-    no("out bf16", torch.ops.kgc.kv4_read, torch.zeros(3, 2, d, device=gpu), kc, pos)
+    no("slots int64", ops.kv4_read, kc, pos.int(), bf)
+    no("bf16 / fp16", ops.kv4_read, kc, pos, torch.float32)
+    no("4-bit cache", ops.kv4_read, kc[..., :60].contiguous(), pos, bf)
