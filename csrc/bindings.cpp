@@ -488,6 +488,7 @@ void prefill_attention(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Ten
       a.part_o = partials->data_ptr<float>();
       a.part_ml = a.part_o + rows * a.Z * q.size(2);
     }
+    TORCH_CHECK(work_seq.numel() * q.size(1) * a.Z < ((int64_t)1 << 31), "grid");
     a.q = q.data_ptr();
     a.k_cache = k_cache.data_ptr();
     a.v_cache = v_cache.data_ptr();

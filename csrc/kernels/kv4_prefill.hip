@@ -25,11 +25,13 @@ __device__ __forceinline__ float kv4_max_pair(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// Where 16-byte chunk c of a tile's row lies: at c ^ swz(row).  Of K, 16 rows' same chunk is read at a time; of V, 4 rows'
-// four chunks; and 4 rows' same chunk of every quarter is written.  All three then touch all banks once.  (With rows padded by
-// 16 and 32 bytes instead, conflicts took 40 % of the LDS's busy cycles.)
-template <int D> __device__ __forceinline__ int kv4_kswz(int row) { return D == 128 ? row & 15 : row >> 1 & 7; }
-template <int D> __device__ __forceinline__ int kv4_vswz(int row) { return 5 * (D == 128 ? row & 3 : row >> 1 & 1); }
+// l + the two numbers of T in w
+template <typename T> __device__ __forceinline__ float kv4_add_pair(uint32_t w, float l) {
+  if constexpr (std::is_same_v<T, bf16>)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), bf16x2_t{(bf16)1.f, (bf16)1.f}, l, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), f16x2_t{(f16)1.f, (f16)1.f}, l, false);
+}
 
 template <typename T, int D, int GH>
 __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
@@ -40,15 +42,21 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
   typedef typename Vec8<T>::type V8;
   constexpr int QB = KV4_BM / GH;                    // query rows of a workgroup
   constexpr int KS = D / 16, DT = D / 32, W = D / 32; // W: words of a thread's quarter row
-  constexpr int TILE = KV4_BN * D;
-  __shared__ __attribute__((aligned(16))) T lds_k[2][TILE], lds_v[2][TILE];
-  const int seq = work_seq[blockIdx.x], mb = work_mblk[blockIdx.x];
-  const int G = nq / nkv, h = blockIdx.y / (G / GH), head0 = h * G + blockIdx.y % (G / GH) * GH;
+  // Rows of the LDS tiles, padded: of K, 16 rows' same chunk touches all banks, of V, four rows' 32 bytes.  (Chunks swizzled
+  // instead halve the conflicts, 40 % of the LDS's busy cycles; the exclusive ors cost more.)
+  constexpr int KST = D + 8, VST = D + 16;
+  __shared__ __attribute__((aligned(16))) T lds_k[2][KV4_BN * KST], lds_v[2][KV4_BN * VST];
+  // The list's items have most keys first, and so have their blocks here; neighbours, which XCDs take in turn, are the head
+  // groups, so that with a multiple of 8 of them an XCD's cache has one group's pages.
+  const int G = nq / nkv, groups = nkv * (G / GH), rest = blockIdx.x / groups, group = blockIdx.x % groups;
+  const int slice = rest % Z, sub = GH - 1 - rest / Z % GH, item = rest / Z / GH;
+  const int seq = work_seq[item], mb = work_mblk[item];
+  const int h = group / (G / GH), head0 = h * G + group % (G / GH) * GH;
   const int q0 = qsl[seq], qlen = qsl[seq + 1] - q0;
   int L_in = seq_lens[seq];
   KGC_DCHECK_RANGE(L_in, 0, (bt_stride << bs_log2) + 1, "prefill seq_len");
   const int L = min(L_in, bt_stride << bs_log2), ctx0 = L - qlen;
-  const int qbase = mb * KV4_BM + blockIdx.z % GH * QB, slice = blockIdx.z / GH;
+  const int qbase = mb * KV4_BM + sub * QB;
   if (qlen <= 0 || ctx0 < 0 || qbase >= qlen) return;  // the whole workgroup
   const int* bt = block_tables + (int64_t)seq * bt_stride;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, hi = lane >> 5;
@@ -60,32 +68,37 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
   // no row of this wave sees further (it may have none)
   const int wave_tiles = wrow < qlen ? (ctx0 + min(wrow + 32, qlen) - 1) / KV4_BN + 1 : 0;
 
-  const int tok = tid >> 2, part = tid & 3;            // of the tile's rows
+  // A wave loads 16 tokens of a tile, which lie in one page; tokens behind the last one are that one again, and masked.
+  const int tok = tid >> 2, part = tid & 3;
+  const int wv = __builtin_amdgcn_readfirstlane(wave);
   uint32_t kw[W], vw[W];
   uint8_t ks, vs;
-  auto page_of = [&](int kt) { return kgc_bt(bt, min(kt * KV4_BN + tok, L - 1) >> bs_log2, bt_stride, num_blocks); };
-  auto load = [&](int kt, int pg) {                    // tokens behind the last one are that one again, and masked
-    const int64_t page = ((int64_t)pg * nkv + h) * page_bytes;
-    const int row = min(kt * KV4_BN + tok, L - 1) & bsm;
-    const int at = row * (D / 2) + part * (D / 8), sc = bs * (D / 2) + row * (D / 32) + (part * D / 4) / 32;
+  auto base_of = [&](int kt) { return min(kt * KV4_BN + 16 * wv, (L - 1) & ~15); };
+  auto page_of = [&](int kt) { return kgc_bt(bt, base_of(kt) >> bs_log2, bt_stride, num_blocks); };
+  auto load = [&](int kt, int pg) {
+    const int base = base_of(kt);
+    const int64_t page = ((int64_t)pg * nkv + h) * page_bytes + (base & bsm) * (D / 2);
+    const int64_t scales = ((int64_t)pg * nkv + h) * page_bytes + bs * (D / 2) + (base & bsm) * (D / 32);
+    const int row = min(lane >> 2, L - 1 - base);
+    const uint32_t at = row * (D / 2) + part * (D / 8), sc = row * (D / 32) + (part * D / 4) / 32;
     if constexpr (W == 4) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(kc + page + at), y = *reinterpret_cast<const u32x4*>(vc + page + at);
+      const u32x4 x = *reinterpret_cast<const u32x4*>((kc + page) + at), y = *reinterpret_cast<const u32x4*>((vc + page) + at);
 #pragma unroll
       for (int i = 0; i < 4; ++i) { kw[i] = x[i]; vw[i] = y[i]; }
     } else {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(kc + page + at), y = *reinterpret_cast<const u32x2*>(vc + page + at);
+      const u32x2 x = *reinterpret_cast<const u32x2*>((kc + page) + at), y = *reinterpret_cast<const u32x2*>((vc + page) + at);
 #pragma unroll
       for (int i = 0; i < 2; ++i) { kw[i] = x[i]; vw[i] = y[i]; }
     }
-    ks = kc[page + sc];
-    vs = vc[page + sc];
+    ks = (kc + scales)[sc];
+    vs = (vc + scales)[sc];
   };
   auto store = [&](int buf) {
     const float a = kv4_scale(ks), b = kv4_scale(vs);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      *reinterpret_cast<u32x4*>(&lds_k[buf][tok * D + 8 * ((part * W + i) ^ kv4_kswz<D>(tok))]) = fp4x8_widen<T>(kw[i], a);
-      *reinterpret_cast<u32x4*>(&lds_v[buf][tok * D + 8 * ((part * W + i) ^ kv4_vswz<D>(tok))]) = fp4x8_widen<T>(vw[i], b);
+      *reinterpret_cast<u32x4*>(&lds_k[buf][tok * KST + part * (D / 4) + 8 * i]) = fp4x8_widen<T>(kw[i], a);
+      *reinterpret_cast<u32x4*>(&lds_v[buf][tok * VST + part * (D / 4) + 8 * i]) = fp4x8_widen<T>(vw[i], b);
     }
   };
 
@@ -106,8 +119,6 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
   }
   store(0);
   __syncthreads();
-  // this lane's part of a transposing read: row vr of four, 16-byte chunk vq of four
-  const int vr = (lane & 15) >> 2, vq = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
   f32x16 o[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t)
@@ -131,7 +142,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
           Pack8<T> kf;
-          kf.u = *reinterpret_cast<const u32x4*>(K + (32 * g + col) * D + 8 * ((2 * j + hi) ^ kv4_kswz<D>(col)));
+          kf.u = *reinterpret_cast<const u32x4*>(K + (32 * g + col) * KST + 16 * j + 8 * hi);
           s[g] = mfma32x32x16(kf.v, qf[j], s[g]);
         }
       }
@@ -147,7 +158,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[g][i]);
+        for (int i = 0; i < 16; ++i) top = __builtin_elementwise_maximum(top, s[g][i]);   // (fmaxf quiets every score first)
       top = kv4_max_pair(top) * scale_log2;
       // the maximum moves only where it grows by more than 8: probabilities are then at most 2^8, and O is seldom rescaled
       if (__any(top > m + 8.f)) {
@@ -166,18 +177,19 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
           Pack8<T> p;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g][8 * j + i], scale_log2, -ref));
-            l += e;
-            p.h[i] = from_f<T>(e);                     // at most 2^8; the sum keeps 32 bits
+            // at most 2^8, rounded to T for the product; the sum, in 32 bits, is that of the rounded ones
+            p.h[i] = from_f<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[g][8 * j + i], scale_log2, -ref)));
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) l = kv4_add_pair<T>(p.u[i], l);
           pf[2 * g + j] = p.v;
         }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-          const T* src = V + (16 * j + 4 * hi + vr) * D + 8 * ((4 * t + vq) ^ kv4_vswz<D>(vr)) + 4 * (lane & 1);
-          const u32x2 a = ld_tr4(src), b = ld_tr4(src + 8 * D);
+          const T* src = V + (16 * j + 4 * hi + ((lane & 15) >> 2)) * VST + 32 * t + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+          const u32x2 a = ld_tr4(src), b = ld_tr4(src + 8 * VST);
           Pack8<T> vf;
           vf.u = u32x4{a.x, a.y, b.x, b.y};
           o[t] = mfma32x32x16(vf.v, pf[j], o[t]);
@@ -251,7 +263,7 @@ template <typename T, int D>
 static void kv4_prefill_dispatch(const Kv4Prefill& a, float sl2, hipStream_t s) {
   const int G = a.nq / a.nkv;
 #define KGC_KV4_PF(GH)                                                                                                \
-  kv4_prefill_kernel<T, D, GH><<<dim3(a.n_work, a.nkv * (G / GH), GH * a.Z), 256, 0, s>>>(                                     \
+  kv4_prefill_kernel<T, D, GH><<<a.n_work * (a.nkv * (G / GH) * GH * a.Z), 256, 0, s>>>(                                     \
       (const T*)a.q, (T*)a.out, (const uint8_t*)a.k_cache, (const uint8_t*)a.v_cache, a.block_tables, a.bt_stride,      \
       a.query_start_loc, a.seq_lens, a.work_seq, a.work_mblk, a.nq, a.nkv, a.bs_log2, sl2, a.num_blocks,        \
       a.part_o, a.part_ml, a.Z)
