@@ -87,22 +87,20 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_decode_kernel(
   f32x4 o[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Pack8<T> qf[KS];
+  const T* qrow = q + ((int64_t)b * nq + h * G + (r16 < G ? r16 : 0)) * D + qd * (D / 4);
+#pragma unroll
+  for (int s = 0; s < KS; ++s) qf[s].u = *reinterpret_cast<const u32x4*>(qrow + 8 * s);
   Frag fa, fb;
   if (c0 < c1) {
     issue(fa, c0);
     issue(fb, min(c0 + 1, c1 - 1));
   }
-  V8 qf[KS];
-  {
-    const bool valid = r16 < G;
-    const T* qrow = q + ((int64_t)b * nq + h * G + (valid ? r16 : 0)) * D + qd * (D / 4);
+  // q is there before the loop: a wait for it in there would be one for the newest chunk's loads, too
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      Pack8<T> t;
-      t.u = *reinterpret_cast<const u32x4*>(qrow + 8 * s);
-      if (!valid) t.u = u32x4{0, 0, 0, 0};
-      qf[s] = t.v;
-    }
+  for (int s = 0; s < KS; ++s) {
+    asm volatile("" : "+v"(qf[s].u));
+    if (r16 >= G) qf[s].u = u32x4{0, 0, 0, 0};
   }
   auto compute = [&](const Frag& f, int ci) {
     const int base = ci << 5;
@@ -115,7 +113,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_decode_kernel(
       for (int s = 0; s < KS; ++s) {
         Pack8<T> kf;
         kf.u = fp4x8_widen<T>(f.k[g][s], size);
-        sc[g] = mfma16x16x32(kf.v, qf[s], sc[g]);
+        sc[g] = mfma16x16x32(kf.v, qf[s].v, sc[g]);
       }
     }
 #pragma unroll

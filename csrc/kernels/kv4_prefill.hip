@@ -1,10 +1,9 @@
 // Causal attention of a step's prompt rows over the 4-bit cache (kv4.h): fresh prompts and chunks that continue one.
 //
-// A workgroup of 4 waves has 32 query rows of each of GH heads of one kv head (GH = 1, 2, 4; GH * 32 of the 128-row work item's
-// rows with 4 / GH of its blocks).  Keys and values advance in tiles of 64 tokens: a thread loads a quarter row of K and
-// of V (D / 8 bytes each) while the tile before it computes, widens them and writes them to LDS as T, in two buffers, one
-// barrier per tile.  So a tile is widened once for 128 rows of queries, and a wave widens D / 32 * 4 instructions' worth of it beside
-// its own 4 * D / 8 MFMAs.
+// A workgroup of 4 waves has 32 query rows of each of GH heads of one kv head (GH = 4: 32 rows of the 128-row work item, 2: 64,
+// 1: 128).  Keys and values advance in tiles of 64 tokens: a thread loads a quarter row of K and of V (D / 8 bytes each) while
+// the tile before it computes, widens them and writes them to LDS as T.  So a tile is widened once for 128 rows of queries:
+// 32 conversions a wave beside the 32 MFMAs of 32 cycles that it feeds (D = 128).
 //
 // v_mfma_f32_32x32x16: S^T = K Q^T and O^T = V^T P^T, so that a query is a lane's column in every accumulator: its maximum
 // and sum are the lane's own (and its partner's, lane ^ 32), and S^T's accumulator, packed, is the B operand of the second product.
@@ -12,8 +11,14 @@
 //
 // Z > 1: few rows after long contexts leave CUs idle, so that Z workgroups share an item's tiles; each leaves its rows' maximum,
 // sum and unnormalised result, which kv4_prefill_merge_kernel joins.
+//
+// 4 x 4096 rows of 32 / 8 heads of 128 take 522 us (1.03 PFLOP/s; a large matrix product reaches 1.40): the matrix cores work in half
+// of a CU's busy cycles, vector instructions issue in 46 %, a wave's own products and softmax one after the other.  Scores of the
+// next tile beside this one's softmax need 32 registers more, which the compiler takes from elsewhere: with 64 keys at a time
+// they spill (1320 us), with 32 keys it is 678 us, and 760 with the order prescribed.
 #include "common.h"
 #include "kv4.h"
+#include "device.h"
 #include "launch.h"
 
 namespace kgc {
@@ -33,8 +38,8 @@ template <typename T> __device__ __forceinline__ float kv4_add_pair(uint32_t w, 
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), f16x2_t{(f16)1.f, (f16)1.f}, l, false);
 }
 
-template <typename T, int D, int GH>
-__global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
+template <typename T, int D, int GH, int BUFS>
+__global__ __launch_bounds__(256, BUFS == 2 ? 2 : D == 128 ? 3 : 4) void kv4_prefill_kernel(
     const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
     const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ qsl, const int* __restrict__ seq_lens,
     const int* __restrict__ work_seq, const int* __restrict__ work_mblk, int nq, int nkv, int bs_log2, float scale_log2,
@@ -45,7 +50,7 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
   // Rows of the LDS tiles, padded: of K, 16 rows' same chunk touches all banks, of V, four rows' 32 bytes.  (Chunks swizzled
   // instead halve the conflicts, 40 % of the LDS's busy cycles; the exclusive ors cost more.)
   constexpr int KST = D + 8, VST = D + 16;
-  __shared__ __attribute__((aligned(16))) T lds_k[2][KV4_BN * KST], lds_v[2][KV4_BN * VST];
+  __shared__ __attribute__((aligned(16))) T lds_k[BUFS][KV4_BN * KST], lds_v[BUFS][KV4_BN * VST];
   // The list's items have most keys first, and so have their blocks here; neighbours, which XCDs take in turn, are the head
   // groups, so that with a multiple of 8 of them an XCD's cache has one group's pages.
   const int G = nq / nkv, groups = nkv * (G / GH), rest = blockIdx.x / groups, group = blockIdx.x % groups;
@@ -102,22 +107,19 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
     }
   };
 
+  // Lane (row col, hi) has elements 16 s + 8 hi .. + 7; rows behind the prompt's last one are that one again, not stored
+  const int qi = min(wrow + col, qlen - 1), qpos = ctx0 + qi;
+  Pack8<T> qf[KS];
+  const T* qrow = q + ((int64_t)(q0 + qi) * nq + head) * D + 8 * hi;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) qf[s].u = *reinterpret_cast<const u32x4*>(qrow + 16 * s);
   int pg = page_of(first);                             // (an empty slice: a tile that is there, not used)
   load(first, pg);
   pg = page_of(first + 1);
-  // q: lane (row col, hi) has elements 16 s + 8 hi .. + 7; rows behind the prompt's last one are that one again, not stored
-  const int qi = min(wrow + col, qlen - 1), qpos = ctx0 + qi;
-  V8 qf[KS];
-  {
-    const T* qrow = q + ((int64_t)(q0 + qi) * nq + head) * D + 8 * hi;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      Pack8<T> t;
-      t.u = *reinterpret_cast<const u32x4*>(qrow + 16 * s);
-      qf[s] = t.v;
-    }
-  }
   store(0);
+  // q is there before the loop: a wait for it in there would be one for the next tile's loads, too
+#pragma unroll
+  for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s].u));
   __syncthreads();
   f32x16 o[DT];
 #pragma unroll
@@ -126,26 +128,26 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
     for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
   float m = -INFINITY, l = 0.f;
   for (int kt = first; kt < tiles; ++kt) {
-    const int buf = (kt - first) & 1;
     if (kt + 1 < tiles) {
       load(kt + 1, pg);
       pg = page_of(kt + 2);
     }
     if (kt < wave_tiles) {
-      const T* K = lds_k[buf];
-      const T* V = lds_v[buf];
+      const T* K = lds_k[BUFS == 2 ? kt - first & 1 : 0];
+      const T* V = lds_v[BUFS == 2 ? kt - first & 1 : 0];
       f32x16 s[2];
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
+      for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[g][i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < KS; ++j) {
+      for (int j = 0; j < KS; ++j)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
           Pack8<T> kf;
           kf.u = *reinterpret_cast<const u32x4*>(K + (32 * g + col) * KST + 16 * j + 8 * hi);
-          s[g] = mfma32x32x16(kf.v, qf[j], s[g]);
+          s[g] = mfma32x32x16(kf.v, qf[j].v, s[g]);
         }
-      }
       const int key0 = kt * KV4_BN + 4 * hi;           // element i of half g: key0 + 32 g + 8 (i / 4) + i % 4
       if (kt * KV4_BN + KV4_BN - 1 > ctx0 + wrow) {    // some row of the wave does not see all of the tile
 #pragma unroll
@@ -196,7 +198,8 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
         }
     }
     if (kt + 1 < tiles) {
-      store(buf ^ 1);
+      if constexpr (BUFS == 1) __syncthreads();
+      store(BUFS == 2 ? kt - first + 1 & 1 : 0);
       __syncthreads();
     }
   }
@@ -229,50 +232,73 @@ __global__ __launch_bounds__(256, 2) void kv4_prefill_kernel(
     }
 }
 
-// A wave per row of the work items' blocks and heads: lane z has slice z's maximum and sum.
+// D / 4 threads per row of a work item's block and head, four elements each; slices' partials eight at a time.
 constexpr int KV4_MAX_SLICES = 32;
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(
     T* __restrict__ out, const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ qsl,
     const int* __restrict__ seq_lens, const int* __restrict__ work_seq, const int* __restrict__ work_mblk, int nq, int cap,
     int Z) {
-  const int seq = work_seq[blockIdx.x], q0 = qsl[seq], qlen = qsl[seq + 1] - q0;
-  const int lane = threadIdx.x & 63, r = work_mblk[blockIdx.x] * KV4_BM + blockIdx.z * 4 + (threadIdx.x >> 6);
+  constexpr int ROWS = 256 / (D / 4), ZB = 8;
+  const int item = blockIdx.x / nq, head = blockIdx.x % nq;
+  const int seq = work_seq[item], q0 = qsl[seq], qlen = qsl[seq + 1] - q0;
+  const int r = work_mblk[item] * KV4_BM + blockIdx.y * ROWS + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
   if (r >= qlen || min(seq_lens[seq], cap) < qlen) return;    // as the kernel above
-  const int64_t row = (int64_t)(q0 + r) * nq + blockIdx.y;
-  const float m = lane < Z ? part_ml[2 * (row * Z + lane)] : -INFINITY;
-  const float l = lane < Z ? part_ml[2 * (row * Z + lane) + 1] : 0.f;
-  const float top = wave_max(m), w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-  const float total = wave_sum(w == 0.f ? 0.f : w * l);
-  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
-  constexpr int E = D / 64;
-  float acc[E];
+  const int64_t row = ((int64_t)(q0 + r) * nq + head) * Z;
+  float top = -INFINITY, total = 0.f;
+  for (int z = 0; z < Z; ++z) top = fmaxf(top, part_ml[2 * (row + z)]);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int z0 = 0; z0 < Z; z0 += ZB) {
+    float m[ZB], l[ZB];
+    f32x4 v[ZB];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int z = 0; z < Z; ++z) {
-    const float f = __shfl(w, z, 64);
-    if (f == 0.f) continue;                                  // nothing seen there, or nothing that counts
+    for (int i = 0; i < ZB; ++i) {
+      const int z = min(z0 + i, Z - 1);
+      m[i] = part_ml[2 * (row + z)];
+      l[i] = part_ml[2 * (row + z) + 1];
+      v[i] = *reinterpret_cast<const f32x4*>(part_o + (row + z) * D + d);
+    }
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += f * part_o[(row * Z + z) * D + lane * E + e];
+    for (int i = 0; i < ZB; ++i) {
+      // a slice that saw nothing has zeros; one that saw a NaN has m = inf, and its row is NaN
+      const float f = z0 + i < Z && m[i] != -INFINITY ? __builtin_amdgcn_exp2f(m[i] - top) : 0.f;
+      total += f * l[i];
+      acc += v[i] * f;
+    }
   }
+  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  Pack4<T> pk;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[row * D + lane * E + e] = from_f<T>(acc[e] * inv);
+  for (int i = 0; i < 4; ++i) pk.h[i] = from_f<T>(acc[i] * inv);
+  *reinterpret_cast<u32x2*>(out + row / Z * D + d) = pk.u;
 }
 
 template <typename T, int D>
 static void kv4_prefill_dispatch(const Kv4Prefill& a, float sl2, hipStream_t s) {
   const int G = a.nq / a.nkv;
-#define KGC_KV4_PF(GH)                                                                                                \
-  kv4_prefill_kernel<T, D, GH><<<a.n_work * (a.nkv * (G / GH) * GH * a.Z), 256, 0, s>>>(                                     \
+  // One buffer per tile: three workgroups of heads of 128 fit a CU (four of 64), which fill each other's waits; two, and a barrier less
+  // per tile, where there are not more workgroups than two per CU: two buffers -> one, us: 4 x 4096 543 -> 522, 32 x 512 121.5 ->
+  // 113; 64 rows alone 6.2 -> 6.9, 512 18.0 -> 19.5, 2048 55 -> 61.
+#define KGC_KV4_PF_B(GH, BUFS)                                                                                        \
+  kv4_prefill_kernel<T, D, GH, BUFS><<<blocks, 256, 0, s>>>(                                                            \
       (const T*)a.q, (T*)a.out, (const uint8_t*)a.k_cache, (const uint8_t*)a.v_cache, a.block_tables, a.bt_stride,      \
-      a.query_start_loc, a.seq_lens, a.work_seq, a.work_mblk, a.nq, a.nkv, a.bs_log2, sl2, a.num_blocks,        \
-      a.part_o, a.part_ml, a.Z)
-  if (G % 4 == 0) KGC_KV4_PF(4);
-  else if (G % 2 == 0) KGC_KV4_PF(2);
-  else KGC_KV4_PF(1);
+      a.query_start_loc, a.seq_lens, a.work_seq, a.work_mblk, a.nq, a.nkv, a.bs_log2, sl2, a.num_blocks, a.part_o,      \
+      a.part_ml, a.Z)
+#define KGC_KV4_PF(GH)                                                                                                \
+  const int blocks = a.n_work * (a.nkv * (G / GH) * GH * a.Z);                                                          \
+  if (blocks <= 2 * device_cus()) KGC_KV4_PF_B(GH, 2);                                                                  \
+  else KGC_KV4_PF_B(GH, 1)
+  if (G % 4 == 0) {
+    KGC_KV4_PF(4);
+  } else if (G % 2 == 0) {
+    KGC_KV4_PF(2);
+  } else {
+    KGC_KV4_PF(1);
+  }
+#undef KGC_KV4_PF_B
 #undef KGC_KV4_PF
   if (a.Z > 1)
-    kv4_prefill_merge_kernel<T, D><<<dim3(a.n_work, a.nq, KV4_BM / 4), 256, 0, s>>>(
+    kv4_prefill_merge_kernel<T, D><<<dim3(a.n_work * a.nq, KV4_BM / (1024 / D)), 256, 0, s>>>(
         (T*)a.out, a.part_o, a.part_ml, a.query_start_loc, a.seq_lens, a.work_seq, a.work_mblk, a.nq,
         a.bt_stride << a.bs_log2, a.Z);
 }

@@ -381,15 +381,17 @@ def prefill_work_list(query_lens: list[int], seq_lens: list[int]) -> tuple[list[
     return [i for _, i, _ in items], [m for _, _, m in items]
 
 
-def kv4_prefill_slices(rows: int, items: int, seqs: int, num_heads: int, num_kv_heads: int, max_len: int) -> int:
+def kv4_prefill_slices(rows: int, seqs: int, num_heads: int, num_kv_heads: int, head_dim: int, max_len: int) -> int:
     """Workgroups that share the keys of each item of a prompt step over a 4-bit cache (csrc/kernels/kv4_prefill.hip): as
-    many as fill the CUs twice, each with 4 tiles of 64 keys or more."""
-    if os.environ.get("KV4_PZ"):
-        return int(os.environ["KV4_PZ"])
+    many as give each CU two of them (three with heads of 64), with four tiles of 64 keys or more each.  One -> several,
+    us: 3 x 301 after 7000, 12 heads of 64, 113 -> 40 (eight); 8 kv heads of 128, 300 after 2000 54 -> 36, 20 after 8000 171 -> 23,
+    16 x 30 after 1000 41 -> 34, 1000 after 4000 110 -> 98.  The merge takes 4 to 8 us, so that short prompts have one: 512
+    17.4 -> 26."""
     g = num_heads // num_kv_heads
     heads = 4 if g % 4 == 0 else 2 if g % 2 == 0 else 1
-    blocks = min(items * heads, rows * heads // PREFILL_BLOCK_M + seqs) * (num_heads // heads)
-    return max(1, min(512 // max(blocks, 1), math.ceil(max_len / 64) // 4, 32))
+    blocks = seqs * math.ceil(rows / max(seqs, 1) * heads / PREFILL_BLOCK_M) * (num_heads // heads)
+    tiles = math.ceil(max_len / 64)
+    return 1 if tiles < 12 else max(1, min((512 if head_dim == 128 else 768) // max(blocks, 1), tiles // 4, 16))
 
 
 def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -413,8 +415,8 @@ def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         out = torch.empty_like(q)
     partials = None
     if k_cache.dtype == torch.uint8:
-        z = kv4_prefill_slices(q.shape[0], work_seq.shape[0], block_tables.shape[0], q.shape[1], k_cache.shape[1],
-                               max_len or block_tables.shape[1] * k_cache.shape[2])
+        z = kv4_prefill_slices(q.shape[0], block_tables.shape[0], q.shape[1], k_cache.shape[1],
+                               q.shape[2], max_len or block_tables.shape[1] * k_cache.shape[2])
         if z > 1:
             partials = torch.empty(z * q.numel() // q.shape[2] * (q.shape[2] + 2), dtype=torch.float32, device=q.device)
     _k().prefill_attention(out, q, k_cache, v_cache, block_tables, query_start_loc, seq_lens,
