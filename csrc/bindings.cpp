@@ -221,6 +221,8 @@ void check_kv4_attention(const Tensor& q, const Tensor& out, const Tensor& k_cac
   check_kv4(k_cache, v_cache, nkv, q.size(2), q);
   no_kv4_scale(k_scale, v_scale);
   TORCH_CHECK(nq % nkv == 0 && nq / nkv <= 16, "GQA group must be <= 16");
+  TORCH_CHECK(k_cache.size(0) >= 1 || q.size(0) == 0, "4-bit cache: no pages");
+  TORCH_CHECK(q.size(0) < ((int64_t)1 << 31), "rows");
   TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out");
   check_same_dev(q, out, "out");
   TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
@@ -500,6 +502,8 @@ void prefill_attention(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Ten
     a.work_mblk = work_mblk.data_ptr<int>();
     a.bt_stride = (int)block_tables.size(1);
     a.n_work = (int)work_seq.numel();
+    a.seqs = (int)P;
+    a.rows = (int)q.size(0);
     a.nq = (int)q.size(1);
     a.nkv = (int)k_cache.size(1);
     a.D = (int)q.size(2);

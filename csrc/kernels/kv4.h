@@ -12,6 +12,11 @@ namespace kgc {
 
 __host__ __device__ __forceinline__ int64_t kv4_page_bytes(int bs, int d) { return (int64_t)bs * (d / 2 + d / 32); }
 
+// page of a block table's entry: one that is no page of the pool gives wrong results, never a fault
+__device__ __forceinline__ int kv4_page(const int* bt, int i, int bt_stride, int num_blocks) {
+  return min(max(kgc_bt(bt, i, bt_stride, num_blocks), 0), num_blocks - 1);
+}
+
 // elements 2 * SEL, 2 * SEL + 1 of the 8 in w, times the scale
 template <typename T, int SEL> __device__ __forceinline__ uint32_t fp4x2_widen(uint32_t w, float scale) {
   if constexpr (std::is_same_v<T, bf16>)

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_decode_kernel(
     for (int g = 0; g < 2; ++g) {
       // tokens behind the slice's last one are that one again: their scores are masked
       const int t0 = min((ci << 5) + 16 * g, end - 1), tok = min((ci << 5) + 16 * g + r16, end - 1);
-      const int64_t page = ((int64_t)kgc_bt(bt, t0 >> bs_log2, bt_stride, num_blocks) * nkv + h) * page_bytes;
+      const int64_t page = ((int64_t)kv4_page(bt, t0 >> bs_log2, bt_stride, num_blocks) * nkv + h) * page_bytes;
       const int row = tok & bsm;
       const int at = row * (D / 2) + qd * (D / 8), sc = bs * (D / 2) + row * (D / 32) + (qd * D / 4) / 32;
       load(f.k[g], kc + page + at);

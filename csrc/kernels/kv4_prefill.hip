@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256, BUFS == 2 ? 2 : D == 128 ? 3 : 4) void kv4_pre
     const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
     const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ qsl, const int* __restrict__ seq_lens,
     const int* __restrict__ work_seq, const int* __restrict__ work_mblk, int nq, int nkv, int bs_log2, float scale_log2,
-    int num_blocks, float* __restrict__ part_o, float* __restrict__ part_ml, int Z) {
+    int num_blocks, int seqs, int rows_all, float* __restrict__ part_o, float* __restrict__ part_ml, int Z) {
   typedef typename Vec8<T>::type V8;
   constexpr int QB = KV4_BM / GH;                    // query rows of a workgroup
   constexpr int KS = D / 16, DT = D / 32, W = D / 32; // W: words of a thread's quarter row
@@ -57,12 +57,13 @@ __global__ __launch_bounds__(256, BUFS == 2 ? 2 : D == 128 ? 3 : 4) void kv4_pre
   const int slice = rest % Z, sub = GH - 1 - rest / Z % GH, item = rest / Z / GH;
   const int seq = work_seq[item], mb = work_mblk[item];
   const int h = group / (G / GH), head0 = h * G + group % (G / GH) * GH;
+  if (seq < 0 || seq >= seqs || mb < 0) return;        // the whole workgroup, and so below
   const int q0 = qsl[seq], qlen = qsl[seq + 1] - q0;
   int L_in = seq_lens[seq];
   KGC_DCHECK_RANGE(L_in, 0, (bt_stride << bs_log2) + 1, "prefill seq_len");
   const int L = min(L_in, bt_stride << bs_log2), ctx0 = L - qlen;
   const int qbase = mb * KV4_BM + sub * QB;
-  if (qlen <= 0 || ctx0 < 0 || qbase >= qlen) return;  // the whole workgroup
+  if (q0 < 0 || qlen <= 0 || qlen > rows_all - q0 || ctx0 < 0 || qbase >= qlen) return;
   const int* bt = block_tables + (int64_t)seq * bt_stride;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, hi = lane >> 5;
   const int bs = 1 << bs_log2, bsm = bs - 1;
@@ -79,7 +80,7 @@ __global__ __launch_bounds__(256, BUFS == 2 ? 2 : D == 128 ? 3 : 4) void kv4_pre
   uint32_t kw[W], vw[W];
   uint8_t ks, vs;
   auto base_of = [&](int kt) { return min(kt * KV4_BN + 16 * wv, (L - 1) & ~15); };
-  auto page_of = [&](int kt) { return kgc_bt(bt, base_of(kt) >> bs_log2, bt_stride, num_blocks); };
+  auto page_of = [&](int kt) { return kv4_page(bt, base_of(kt) >> bs_log2, bt_stride, num_blocks); };
   auto load = [&](int kt, int pg) {
     const int base = base_of(kt);
     const int64_t page = ((int64_t)pg * nkv + h) * page_bytes + (base & bsm) * (D / 2);
@@ -250,12 +251,14 @@ template <typename T, int D>
 __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(
     T* __restrict__ out, const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ qsl,
     const int* __restrict__ seq_lens, const int* __restrict__ work_seq, const int* __restrict__ work_mblk, int nq, int cap,
-    int Z) {
+    int seqs, int rows_all, int Z) {
   constexpr int ROWS = 256 / (D / 4), ZB = 8;
   const int item = blockIdx.x / nq, head = blockIdx.x % nq;
-  const int seq = work_seq[item], q0 = qsl[seq], qlen = qsl[seq + 1] - q0;
-  const int r = work_mblk[item] * KV4_BM + blockIdx.y * ROWS + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-  if (r >= qlen || min(seq_lens[seq], cap) < qlen) return;    // as the kernel above
+  const int seq = work_seq[item], mb = work_mblk[item];
+  if (seq < 0 || seq >= seqs || mb < 0) return;
+  const int q0 = qsl[seq], qlen = qsl[seq + 1] - q0;
+  const int r = mb * KV4_BM + blockIdx.y * ROWS + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  if (q0 < 0 || qlen > rows_all - q0 || r >= qlen || min(seq_lens[seq], cap) < qlen) return;    // as the kernel above
   const int64_t row = ((int64_t)(q0 + r) * nq + head) * Z;
   float top = -INFINITY, total = 0.f;
   for (int z = 0; z < Z; ++z) top = fmaxf(top, part_ml[2 * (row + z)]);
@@ -294,8 +297,8 @@ static void kv4_prefill_dispatch(const Kv4Prefill& a, float sl2, hipStream_t s) 
 #define KGC_KV4_PF_B(GH, BUFS)                                                                                        \
   kv4_prefill_kernel<T, D, GH, BUFS><<<blocks, 256, 0, s>>>(                                                            \
       (const T*)a.q, (T*)a.out, (const uint8_t*)a.k_cache, (const uint8_t*)a.v_cache, a.block_tables, a.bt_stride,      \
-      a.query_start_loc, a.seq_lens, a.work_seq, a.work_mblk, a.nq, a.nkv, a.bs_log2, sl2, a.num_blocks, a.part_o,      \
-      a.part_ml, a.Z)
+      a.query_start_loc, a.seq_lens, a.work_seq, a.work_mblk, a.nq, a.nkv, a.bs_log2, sl2, a.num_blocks, a.seqs,        \
+      a.rows, a.part_o, a.part_ml, a.Z)
 #define KGC_KV4_PF(GH)                                                                                                \
   const int blocks = a.n_work * (a.nkv * (G / GH) * GH * a.Z);                                                          \
   if (blocks <= 2 * device_cus()) KGC_KV4_PF_B(GH, 2);                                                                  \
@@ -312,7 +315,7 @@ static void kv4_prefill_dispatch(const Kv4Prefill& a, float sl2, hipStream_t s) 
   if (a.Z > 1)
     kv4_prefill_merge_kernel<T, D><<<dim3(a.n_work * a.nq, KV4_BM / (1024 / D)), 256, 0, s>>>(
         (T*)a.out, a.part_o, a.part_ml, a.query_start_loc, a.seq_lens, a.work_seq, a.work_mblk, a.nq,
-        a.bt_stride << a.bs_log2, a.Z);
+        a.bt_stride << a.bs_log2, a.seqs, a.rows, a.Z);
 }
 
 void launch_kv4_prefill(int dtype, const Kv4Prefill& a, float scale, hipStream_t s) {

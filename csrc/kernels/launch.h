@@ -108,7 +108,7 @@ struct Kv4Prefill {
   const void *q, *k_cache, *v_cache;
   void* out;
   const int *block_tables, *query_start_loc, *seq_lens, *work_seq, *work_mblk;
-  int bt_stride, n_work, nq, nkv, D, bs_log2, num_blocks;
+  int bt_stride, n_work, seqs, rows, nq, nkv, D, bs_log2, num_blocks;
   float *part_o, *part_ml;   // Z > 1: [rows, nq, Z, D] and [rows, nq, Z, 2]
   int Z;                     // workgroups that share an item's keys, 1 to 32
 };

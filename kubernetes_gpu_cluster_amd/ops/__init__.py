@@ -143,7 +143,8 @@ def rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Ten
     """k_cache / v_cache may be fp8 (torch.float8_e4m3fn): values are stored as
     fp8(x / scale); or 4-bit (uint8, ``kv4_cache_shape``): blocks of 32 elements of a head have a
     power of two of their own (k_scale = v_scale = 1), and k is the code nearest to the exactly
-    rotated key.  ``sections``: positions are int64 [A, T], one row per axis (time, height, width),
+    rotated key; e2m1 has no infinities and no NaN, which are stored as the largest value and zero.
+    Slots are distinct (-1: no write).  ``sections``: positions are int64 [A, T], one row per axis (time, height, width),
     and pair i of a head turns by the axis whose section holds i -- pairs per axis, one after the
     other, head_dim / 2 in all, 4 axes at most; positions outside ``cos_sin`` take its nearest row.
     On the GPU ``qkv`` may also be the K9m split-K slices of the QKV

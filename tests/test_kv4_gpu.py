@@ -307,6 +307,38 @@ def test_nan_queries_stay_with_their_rows(gpu, z):
     assert torch.equal(dec.cpu().isnan().all(-1), bad[4:6]) and torch.equal(dec.cpu().isnan().any(-1), bad[4:6])
 
 
+def test_tables_and_lists_out_of_range(gpu):
+    """Page numbers, lengths and work items that are none: other rows are right, and nothing is read or written
+    elsewhere (the kernels clamp pages and lengths to the pool and leave such items out)."""
+    if ops.DEBUG:
+        pytest.skip("the bounds-checking build reports them")
+    new, old = [20, 40], [100, 300]
+    q, kc, vc, bt, totals = _attention_case(9, 4, 2, 64, 32, torch.bfloat16, new, old)
+    bad = bt.clone()
+    bad[0, 0], bad[0, 2] = -7, 1 << 30
+    a = [t.to(gpu) for t in (kc, vc, bad)]
+    n = torch.tensor(totals, dtype=torch.int32, device=gpu)
+    last = torch.stack([q[19], q[59], q[0]]).to(gpu)
+    bt3 = torch.cat([a[2], a[2][1:]])
+    dec = ops.paged_attention_decode(last, a[0], a[1], bt3, torch.tensor([120, 340, -5], dtype=torch.int32, device=gpu),
+                                     0.125, None, 2)
+    assert not dec[2].any()
+    _check_attention(dec[1:2].cpu(), q[59:], kc, vc, bt[1:], [1], totals[1:], 0.125)
+    ws = torch.tensor([1, 7, -1, 0, 1], dtype=torch.int32, device=gpu)
+    wm = torch.tensor([0, 0, 0, -1, 5], dtype=torch.int32, device=gpu)
+    for z in (1, 4):
+        out = torch.full_like(q, 7).to(gpu)
+        torch.ops.kgc.prefill_attention(out, q.to(gpu), *a, _starts(new).to(gpu), n, ws, wm, 0.125, 1.0, 1.0, 0,
+                                        torch.empty(z * q.numel() // 64 * 66, device=gpu))
+        assert (out[:20] == 7).all()
+        _check_attention(out[20:].cpu(), q[20:], kc, vc, bt[1:], new[1:], totals[1:], 0.125)
+        starts = torch.tensor([-3, 0, 999], dtype=torch.int32, device=gpu)
+        out.fill_(7)
+        torch.ops.kgc.prefill_attention(out, q.to(gpu), *a, starts, n, ws, wm, 0.125, 1.0, 1.0, 0,
+                                        torch.empty(z * q.numel() // 64 * 66, device=gpu))
+        assert (out == 7).all()
+
+
 @pytest.mark.parametrize("dt", DT)
 def test_prompts_sharp_rows(gpu, dt):
     new, old = [150, 40], [90, 0]
@@ -457,6 +489,7 @@ def test_refusals(gpu):
     no("ctx_lens", dec, q, kc, kc, bt, n[:2], 1.0)
     no("different device", dec, q, kc, kc, bt.cpu(), n, 1.0)
     no("different device", dec, q, kc, kc.cpu(), bt, n, 1.0)
+    no("no pages", dec, q, kc[:0], kc[:0], bt, n, 1.0)
     no("query_start_loc", pre, q, kc, kc, bt[:1], n, n[:1], 1.0, n, n)
     no("seq_lens", pre, q, kc, kc, bt[:2], n, n[:1], 1.0, n, n)
     no("work list", pre, q, kc, kc, bt[:2], n, n[:2], 1.0, n, n[:2])
