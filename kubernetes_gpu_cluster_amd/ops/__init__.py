@@ -156,8 +156,7 @@ def rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Ten
                                     use_rope, k_scale, v_scale, sections)
     sl = qkv.dim() == 3
     T = qkv.shape[1] if sl else qkv.shape[0]
-    q = torch.empty(T, num_heads, head_dim, dtype=(dtype or qkv.dtype) if sl else qkv.dtype,
-                    device=qkv.device)
+    q = qkv.new_empty((T, num_heads, head_dim), dtype=(dtype or qkv.dtype) if sl else qkv.dtype)
     _k().rope_kv_write(qkv, positions, cos_sin, q, k_cache, v_cache, slot_mapping, q_norm_w,
                        k_norm_w, num_heads, num_kv_heads, head_dim, eps, use_rope, k_scale,
                        v_scale, None if sections is None else list(sections))
