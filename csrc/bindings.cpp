@@ -329,6 +329,57 @@ static void check_partials(const Tensor& ml, const Tensor& es, const Tensor& tmp
               ": partials on one device");
 }
 
+void kv4_decode_into(const Tensor& out, const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                     const Tensor& block_tables, const Tensor& ctx_lens, const Tensor& max_logits,
+                     const Tensor& exp_sums, const Tensor& tmp_out, int64_t Z, double scale, double k_scale,
+                     double v_scale) {
+  check_kv4_attention(q, out, k_cache, v_cache, block_tables, k_scale, v_scale);
+  const int64_t B = q.size(0), nq = q.size(1), d = q.size(2);
+  TORCH_CHECK(B < ((int64_t)1 << 31) && k_cache.size(1) <= 65535 && nq <= 65535, "grid");
+  TORCH_CHECK(block_tables.size(0) >= B, "block_tables int32 [B, max_blocks]");
+  TORCH_CHECK(ctx_lens.scalar_type() == at::kInt && ctx_lens.is_contiguous() && ctx_lens.numel() >= B, "ctx_lens int32 [B]");
+  check_same_dev(q, ctx_lens, "ctx_lens");
+  check_partials(max_logits, exp_sums, tmp_out, B, nq, d, Z, "kgc.paged_decode");
+  check_same_dev(q, tmp_out, "partials");
+  kgc::Kv4Decode a{};
+  a.q = q.data_ptr();
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v_cache.data_ptr();
+  a.out = out.data_ptr();
+  a.block_tables = block_tables.data_ptr<int>();
+  a.ctx_lens = ctx_lens.data_ptr<int>();
+  a.max_logits = max_logits.data_ptr<float>();
+  a.exp_sums = exp_sums.data_ptr<float>();
+  a.tmp_out = tmp_out.data_ptr<float>();
+  a.bt_stride = (int)block_tables.size(1);
+  a.B = (int)B;
+  a.nq = (int)nq;
+  a.nkv = (int)k_cache.size(1);
+  a.D = (int)d;
+  a.bs_log2 = log2_exact(k_cache.size(2), "block_size");
+  a.Z = (int)Z;
+  a.num_blocks = (int)k_cache.size(0);
+  kgc::launch_kv4_decode(dt_code(q), a, (float)scale, stream());
+}
+
+// as paged_decode over a 4-bit cache, with a result of its own; no partials: its own, too
+Tensor kv4_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor ctx_lens,
+                  std::optional<Tensor> max_logits, std::optional<Tensor> exp_sums, std::optional<Tensor> tmp_out,
+                  int64_t Z, double scale) {
+  check_gpu(q, "q");
+  c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
+  TORCH_CHECK(q.dim() == 3 && q.is_contiguous(), "q [B, nq, d] contiguous");
+  TORCH_CHECK(Z >= 1 && Z <= 1024, "kgc.paged_decode: need 1 <= Z <= 1024");
+  Tensor out = at::empty_like(q);
+  const int64_t rows = q.size(0) * q.size(1) * Z;
+  const auto f32 = q.options().dtype(at::kFloat);
+  Tensor ml = max_logits.has_value() ? *max_logits : at::empty({rows}, f32);
+  Tensor es = exp_sums.has_value() ? *exp_sums : at::empty({rows}, f32);
+  Tensor tmp = tmp_out.has_value() ? *tmp_out : at::empty({rows, q.size(2)}, f32);
+  kv4_decode_into(out, q, k_cache, v_cache, block_tables, ctx_lens, ml, es, tmp, Z, scale, 1.0, 1.0);
+  return out;
+}
+
 void paged_decode(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables,
                   Tensor ctx_lens, Tensor max_logits, Tensor exp_sums, Tensor tmp_out,
                   int64_t Z, double scale, double k_scale, double v_scale) {
@@ -336,33 +387,8 @@ void paged_decode(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor b
   c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
   TORCH_CHECK(q.dim() == 3 && q.is_contiguous(), "q [B, nq, d] contiguous");
   if (k_cache.scalar_type() == at::kByte) {
-    check_kv4_attention(q, out, k_cache, v_cache, block_tables, k_scale, v_scale);
-    const int64_t B = q.size(0), nq = q.size(1), d = q.size(2);
-    TORCH_CHECK(B < ((int64_t)1 << 31) && k_cache.size(1) <= 65535 && nq <= 65535, "grid");
-    TORCH_CHECK(block_tables.size(0) >= B, "block_tables int32 [B, max_blocks]");
-    TORCH_CHECK(ctx_lens.scalar_type() == at::kInt && ctx_lens.is_contiguous() && ctx_lens.numel() >= B, "ctx_lens int32 [B]");
-    check_same_dev(q, ctx_lens, "ctx_lens");
-    check_partials(max_logits, exp_sums, tmp_out, B, nq, d, Z, "kgc.paged_decode");
-    check_same_dev(q, tmp_out, "partials");
-    kgc::Kv4Decode a{};
-    a.q = q.data_ptr();
-    a.k_cache = k_cache.data_ptr();
-    a.v_cache = v_cache.data_ptr();
-    a.out = out.data_ptr();
-    a.block_tables = block_tables.data_ptr<int>();
-    a.ctx_lens = ctx_lens.data_ptr<int>();
-    a.max_logits = max_logits.data_ptr<float>();
-    a.exp_sums = exp_sums.data_ptr<float>();
-    a.tmp_out = tmp_out.data_ptr<float>();
-    a.bt_stride = (int)block_tables.size(1);
-    a.B = (int)B;
-    a.nq = (int)nq;
-    a.nkv = (int)k_cache.size(1);
-    a.D = (int)d;
-    a.bs_log2 = log2_exact(k_cache.size(2), "block_size");
-    a.Z = (int)Z;
-    a.num_blocks = (int)k_cache.size(0);
-    kgc::launch_kv4_decode(dt_code(q), a, (float)scale, stream());
+    kv4_decode_into(out, q, k_cache, v_cache, block_tables, ctx_lens, max_logits, exp_sums, tmp_out, Z, scale, k_scale,
+                    v_scale);
     return;
   }
   const int64_t B = q.size(0), nq = q.size(1), d = q.size(2);
@@ -460,6 +486,68 @@ void paged_decode_rope(Tensor out, Tensor qkv, Tensor positions, Tensor cos_sin,
                                 (float)k_scale, (float)v_scale, (int)k_cache.size(0), stream());
 }
 
+void kv4_prefill_into(const Tensor& out, const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                      const Tensor& block_tables, const Tensor& query_start_loc, const Tensor& seq_lens,
+                      const Tensor& work_seq, const Tensor& work_mblk, double scale, double k_scale, double v_scale,
+                      const std::optional<Tensor>& partials) {
+  check_kv4_attention(q, out, k_cache, v_cache, block_tables, k_scale, v_scale);
+  const int64_t P = block_tables.size(0);
+  TORCH_CHECK(query_start_loc.scalar_type() == at::kInt && query_start_loc.is_contiguous() &&
+              query_start_loc.numel() == P + 1, "query_start_loc");
+  TORCH_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.is_contiguous() && seq_lens.numel() >= P, "seq_lens int32");
+  TORCH_CHECK(work_seq.scalar_type() == at::kInt && work_mblk.scalar_type() == at::kInt && work_seq.is_contiguous() &&
+              work_mblk.is_contiguous() && work_seq.numel() == work_mblk.numel(), "work list");
+  for (const Tensor* t : {&query_start_loc, &seq_lens, &work_seq, &work_mblk}) check_same_dev(q, *t, "prefill operand");
+  TORCH_CHECK(work_seq.numel() <= 2147483647 && q.size(1) <= 65535, "grid");
+  kgc::Kv4Prefill a{};
+  a.Z = 1;
+  if (partials.has_value()) {
+    const int64_t rows = q.size(0) * q.size(1), each = q.size(2) + 2;
+    check_same_dev(q, *partials, "partials");
+    a.Z = (int)std::min<int64_t>(32, rows > 0 ? partials->numel() / (rows * each) : 1);
+    TORCH_CHECK(partials->scalar_type() == at::kFloat && partials->is_contiguous() && a.Z >= 1,
+                "kgc.prefill_attention: partials fp32, rows * heads * (d + 2) for each of 1 to 32 slices");
+    aligned16(*partials, "partials");
+    a.part_o = partials->data_ptr<float>();
+    a.part_ml = a.part_o + rows * a.Z * q.size(2);
+  }
+  TORCH_CHECK(work_seq.numel() * q.size(1) * a.Z < ((int64_t)1 << 31), "grid");
+  a.q = q.data_ptr();
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v_cache.data_ptr();
+  a.out = out.data_ptr();
+  a.block_tables = block_tables.data_ptr<int>();
+  a.query_start_loc = query_start_loc.data_ptr<int>();
+  a.seq_lens = seq_lens.data_ptr<int>();
+  a.work_seq = work_seq.data_ptr<int>();
+  a.work_mblk = work_mblk.data_ptr<int>();
+  a.bt_stride = (int)block_tables.size(1);
+  a.n_work = (int)work_seq.numel();
+  a.seqs = (int)P;
+  a.rows = (int)q.size(0);
+  a.nq = (int)q.size(1);
+  a.nkv = (int)k_cache.size(1);
+  a.D = (int)q.size(2);
+  a.bs_log2 = log2_exact(k_cache.size(2), "block_size");
+  a.num_blocks = (int)k_cache.size(0);
+  kgc::launch_kv4_prefill(dt_code(q), a, (float)scale, stream());
+}
+
+// as prefill_attention over a 4-bit cache, with Z slices and a result of its own
+Tensor kv4_prefill(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor query_start_loc, Tensor seq_lens,
+                   Tensor work_seq, Tensor work_mblk, double scale, int64_t Z) {
+  check_gpu(q, "q");
+  c10::hip::HIPGuardMasqueradingAsCUDA g(q.device());
+  TORCH_CHECK(q.dim() == 3 && q.is_contiguous(), "q [T, nq, d] contiguous");
+  TORCH_CHECK(Z >= 1 && Z <= 32, "kgc.kv4_prefill: 1 to 32 slices");
+  Tensor out = at::empty_like(q);
+  std::optional<Tensor> partials;
+  if (Z > 1) partials = at::empty({q.size(0) * q.size(1) * Z * (q.size(2) + 2)}, q.options().dtype(at::kFloat));
+  kv4_prefill_into(out, q, k_cache, v_cache, block_tables, query_start_loc, seq_lens, work_seq, work_mblk, scale, 1.0, 1.0,
+                   partials);
+  return out;
+}
+
 void prefill_attention(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables,
                        Tensor query_start_loc, Tensor seq_lens, Tensor work_seq,
                        Tensor work_mblk, double scale, double k_scale, double v_scale, int64_t max_len,
@@ -469,47 +557,8 @@ void prefill_attention(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Ten
   TORCH_CHECK(q.dim() == 3 && q.is_contiguous(), "q [T, nq, d] contiguous");
   TORCH_CHECK(!partials.has_value() || k_cache.scalar_type() == at::kByte, "kgc.prefill_attention: partials are for 4-bit caches");
   if (k_cache.scalar_type() == at::kByte) {
-    check_kv4_attention(q, out, k_cache, v_cache, block_tables, k_scale, v_scale);
-    const int64_t P = block_tables.size(0);
-    TORCH_CHECK(query_start_loc.scalar_type() == at::kInt && query_start_loc.is_contiguous() &&
-                query_start_loc.numel() == P + 1, "query_start_loc");
-    TORCH_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.is_contiguous() && seq_lens.numel() >= P, "seq_lens int32");
-    TORCH_CHECK(work_seq.scalar_type() == at::kInt && work_mblk.scalar_type() == at::kInt && work_seq.is_contiguous() &&
-                work_mblk.is_contiguous() && work_seq.numel() == work_mblk.numel(), "work list");
-    for (const Tensor* t : {&query_start_loc, &seq_lens, &work_seq, &work_mblk}) check_same_dev(q, *t, "prefill operand");
-    TORCH_CHECK(work_seq.numel() <= 2147483647 && q.size(1) <= 65535, "grid");
-    kgc::Kv4Prefill a{};
-    a.Z = 1;
-    if (partials.has_value()) {
-      const int64_t rows = q.size(0) * q.size(1), each = q.size(2) + 2;
-      check_same_dev(q, *partials, "partials");
-      a.Z = (int)std::min<int64_t>(32, rows > 0 ? partials->numel() / (rows * each) : 1);
-      TORCH_CHECK(partials->scalar_type() == at::kFloat && partials->is_contiguous() && a.Z >= 1,
-                  "kgc.prefill_attention: partials fp32, rows * heads * (d + 2) for each of 1 to 32 slices");
-      aligned16(*partials, "partials");
-      a.part_o = partials->data_ptr<float>();
-      a.part_ml = a.part_o + rows * a.Z * q.size(2);
-    }
-    TORCH_CHECK(work_seq.numel() * q.size(1) * a.Z < ((int64_t)1 << 31), "grid");
-    a.q = q.data_ptr();
-    a.k_cache = k_cache.data_ptr();
-    a.v_cache = v_cache.data_ptr();
-    a.out = out.data_ptr();
-    a.block_tables = block_tables.data_ptr<int>();
-    a.query_start_loc = query_start_loc.data_ptr<int>();
-    a.seq_lens = seq_lens.data_ptr<int>();
-    a.work_seq = work_seq.data_ptr<int>();
-    a.work_mblk = work_mblk.data_ptr<int>();
-    a.bt_stride = (int)block_tables.size(1);
-    a.n_work = (int)work_seq.numel();
-    a.seqs = (int)P;
-    a.rows = (int)q.size(0);
-    a.nq = (int)q.size(1);
-    a.nkv = (int)k_cache.size(1);
-    a.D = (int)q.size(2);
-    a.bs_log2 = log2_exact(k_cache.size(2), "block_size");
-    a.num_blocks = (int)k_cache.size(0);
-    kgc::launch_kv4_prefill(dt_code(q), a, (float)scale, stream());
+    kv4_prefill_into(out, q, k_cache, v_cache, block_tables, query_start_loc, seq_lens, work_seq, work_mblk, scale, k_scale,
+                     v_scale, partials);
     return;
   }
   const int64_t nq = q.size(1), d = q.size(2);
@@ -3003,6 +3052,10 @@ TORCH_LIBRARY(kgc, m) {
         "Tensor(b!) k_cache, Tensor(c!) v_cache, Tensor slot_mapping, Tensor? q_norm_w, "
         "Tensor? k_norm_w, int nq, int nkv, int d, float eps, bool use_rope, float k_scale=1.0, "
         "float v_scale=1.0, int[]? sections=None) -> ()");
+  m.def("kv4_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor ctx_lens, Tensor(a!)? max_logits, "
+        "Tensor(b!)? exp_sums, Tensor(c!)? tmp_out, int Z, float scale) -> Tensor");
+  m.def("kv4_prefill(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor query_start_loc, "
+        "Tensor seq_lens, Tensor work_seq, Tensor work_mblk, float scale, int Z) -> Tensor");
   m.def("kv4_read(Tensor cache, Tensor slots, ScalarType dtype) -> Tensor");
   m.def("paged_decode(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, "
         "Tensor block_tables, Tensor ctx_lens, Tensor(b!) max_logits, Tensor(c!) exp_sums, "
@@ -3155,6 +3208,8 @@ TORCH_LIBRARY_IMPL(kgc, CUDA, m) {
   m.impl("silu_mul", &silu_mul);
   m.impl("rope_kv_write", &rope_kv_write);
   m.impl("kv4_read", &kv4_read);
+  m.impl("kv4_decode", &kv4_decode);
+  m.impl("kv4_prefill", &kv4_prefill);
   m.impl("paged_decode", &paged_decode);
   m.impl("paged_decode_rope", &paged_decode_rope);
   m.impl("prefill_attention", &prefill_attention);

@@ -309,6 +309,10 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
                                           k_scale, v_scale)
     B, nq, d = q.shape
     if out is None:
+        if k_cache.dtype == torch.uint8 and k_scale == v_scale == 1.0:       # one call, allocations and all
+            ml, es, tmp = workspace or (None, None, None)
+            return _k().kv4_decode(q, k_cache, v_cache, block_tables, context_lens, ml, es, tmp,
+                                   min(grid_z, _decode_z_cap(workspace, B, nq)) if workspace else grid_z, scale)
         out = torch.empty_like(q)
     if workspace is None:
         workspace = decode_partials(B, nq, d, block_tables.shape[1], k_cache.shape[2], q.device)
@@ -387,11 +391,13 @@ def kv4_prefill_slices(rows: int, seqs: int, num_heads: int, num_kv_heads: int, 
     us: 3 x 301 after 7000, 12 heads of 64, 113 -> 40 (eight); 8 kv heads of 128, 300 after 2000 54 -> 36, 20 after 8000 171 -> 23,
     16 x 30 after 1000 41 -> 34, 1000 after 4000 110 -> 98.  The merge takes 4 to 8 us, so that short prompts have one: 512
     17.4 -> 26."""
+    tiles = math.ceil(max_len / 64)
+    if tiles < 12:
+        return 1
     g = num_heads // num_kv_heads
     heads = 4 if g % 4 == 0 else 2 if g % 2 == 0 else 1
     blocks = seqs * math.ceil(rows / max(seqs, 1) * heads / PREFILL_BLOCK_M) * (num_heads // heads)
-    tiles = math.ceil(max_len / 64)
-    return 1 if tiles < 12 else max(1, min((512 if head_dim == 128 else 768) // max(blocks, 1), tiles // 4, 16))
+    return max(1, min((512 if head_dim == 128 else 768) // max(blocks, 1), tiles // 4, 16))
 
 
 def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -411,14 +417,17 @@ def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
         max_len = max(lens, default=0)
         work_seq = torch.tensor(ws, dtype=torch.int32, device=q.device)
         work_mblk = torch.tensor(wm, dtype=torch.int32, device=q.device)
-    if out is None:
-        out = torch.empty_like(q)
     partials = None
     if k_cache.dtype == torch.uint8:
         z = kv4_prefill_slices(q.shape[0], block_tables.shape[0], q.shape[1], k_cache.shape[1],
                                q.shape[2], max_len or block_tables.shape[1] * k_cache.shape[2])
+        if out is None and k_scale == v_scale == 1.0:                        # one call, allocations and all
+            return _k().kv4_prefill(q, k_cache, v_cache, block_tables, query_start_loc, seq_lens, work_seq, work_mblk,
+                                    scale, z)
         if z > 1:
             partials = torch.empty(z * q.numel() // q.shape[2] * (q.shape[2] + 2), dtype=torch.float32, device=q.device)
+    if out is None:
+        out = torch.empty_like(q)
     _k().prefill_attention(out, q, k_cache, v_cache, block_tables, query_start_loc, seq_lens,
                            work_seq, work_mblk, scale, k_scale, v_scale, max_len, partials)
     return out
