@@ -225,6 +225,9 @@ def test_decode(gpu, dt, nq, nkv, d, bs, ctx, z):
                                      torch.tensor(ctx, dtype=torch.int32, device=gpu), d ** -0.5, ws, z, out=out)
     assert got.data_ptr() == out.data_ptr()
     _check_attention(got.cpu(), q, kc, vc, bt, [1] * len(ctx), ctx, d ** -0.5)
+    own = ops.paged_attention_decode(q.to(gpu), kc.to(gpu), vc.to(gpu), bt.to(gpu),
+                                     torch.tensor(ctx, dtype=torch.int32, device=gpu), d ** -0.5, None, z)
+    assert torch.equal(own, got)
 
 
 @pytest.mark.parametrize("dt", DT)
@@ -265,6 +268,9 @@ def test_prompts(gpu, dt, nq, nkv, d, bs, new, old):
                                 torch.tensor(totals, dtype=torch.int32, device=gpu), d ** -0.5, out=out)
     assert got.data_ptr() == out.data_ptr() and (out[-3:] == 7).all()
     _check_attention(got[:-3].cpu(), q, kc, vc, bt, new, totals, d ** -0.5)
+    own = ops.prefill_attention(q.to(gpu), kc.to(gpu), vc.to(gpu), bt.to(gpu), _starts(new).to(gpu),
+                                torch.tensor(totals, dtype=torch.int32, device=gpu), d ** -0.5)
+    _check_attention(own.cpu(), q, kc, vc, bt, new, totals, d ** -0.5)
 
 
 @pytest.mark.parametrize("dt", DT)
@@ -423,6 +429,30 @@ def test_prompt_then_decode(gpu, dt):
         assert ((a.double() - c.double()).abs() <= 3 * torch.finfo(dt).eps * 8).all()
 
 
+def test_pool_beyond_32_bits(gpu):
+    """Pages behind the first 4 GB of a pool: written, read back and attended as in a small one."""
+    g, dt, nq, nkv, d, bs, n = _gen(31), torch.bfloat16, 4, 1, 128, 32, 130
+    nb = (9 << 29) // (bs * ref.kv4_row_bytes(d))             # 4.8 GB each
+    big = [torch.zeros(ops.kv4_cache_shape(nb, nkv, bs, d), dtype=torch.uint8, device=gpu) for _ in range(2)]
+    small = [torch.zeros(ops.kv4_cache_shape(6, nkv, bs, d), dtype=torch.uint8, device=gpu) for _ in range(2)]
+    x = torch.randn(n, (nq + 2 * nkv) * d, generator=g).to(dt).to(gpu)
+    pos = torch.arange(n, device=gpu)
+    table = ref.rope_cos_sin_cache(d, 200, 10000.0).to(gpu)
+    got = []
+    for (kc, vc), first in ((big, nb - 5), (small, 1)):
+        slots = pos + first * bs
+        q = ops.rope_kv_write(x, pos, table, kc, vc, slots, nq, nkv, d)
+        bt = torch.arange(first, first + 5, dtype=torch.int32, device=gpu)[None]
+        ctx = torch.tensor([n], dtype=torch.int32, device=gpu)
+        starts = torch.tensor([0, n], dtype=torch.int32, device=gpu)
+        got.append([q, ops.kv4_read(kc, slots, dt), ops.kv4_read(vc, slots, dt),
+                    ops.prefill_attention(q, kc, vc, bt, starts, ctx, d ** -0.5),
+                    ops.paged_attention_decode(q[-1:], kc, vc, bt, ctx, d ** -0.5, None, 1)])
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and a.any()
+    assert not big[0][:-5].any() and not big[1][:-5].any()
+
+
 def test_on_another_stream(gpu):
     """Work on a stream that is not the default one, behind work that it waits for."""
     q, kc, vc, bt, totals = _attention_case(5, 8, 2, 128, 32, torch.bfloat16, [1] * 4, [600, 31, 32, 5])
@@ -436,8 +466,8 @@ def test_on_another_stream(gpu):
 
 @pytest.mark.parametrize("model", ["tiny-llama", "tiny-qwen3"])
 def test_engine(gpu, model):
-    """--kv-cache-dtype fp4 through the engine: decode by graphs and eagerly give the same greedy tokens, and first
-    tokens are among the five likeliest of the 16-bit cache's run."""
+    """--kv-cache-dtype fp4 through the engine: as long as decode by graphs and eagerly choose the same tokens, their log
+    probabilities differ by the products' rounding; first tokens are among the five likeliest of the 16-bit cache's run."""
     from kubernetes_gpu_cluster_amd.engine.llm_engine import LLM
     from kubernetes_gpu_cluster_amd.engine.sequence import SamplingParams
     prompts = [[5 + i, 6, 7, 8, 9] * 9 for i in range(3)]
@@ -454,6 +484,12 @@ def test_engine(gpu, model):
         llm.shutdown()
     for a, b in zip(outs[0], outs[1]):
         assert b.logprobs[0][0] in [t for t, _ in a.logprobs[0][2]]
+    for a, b in zip(outs[1], outs[2]):
+        for i in range(12):
+            # logits below 8 in bf16, by other products on either side: two roundings of 2^-8 * 8 each
+            assert abs(a.logprobs[i][2][0][1] - b.logprobs[i][2][0][1]) < 0.125
+            if a.output_token_ids[i] != b.output_token_ids[i]:
+                break
 
 
 # ------------------------------------------------------------------ refusals
