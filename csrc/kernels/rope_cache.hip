@@ -224,14 +224,14 @@ __global__ __launch_bounds__(ROPE_NT) void rope_kv_kernel(
 // rows, 8 heads of 128, 134 MB: 75 us, 28 here, the rate of a large copy; fp8 cache, which had the
 // per-token kernel, 86 -> 22).  Up to 1000 rows that do lie with the groups take 4.7 us where blocks
 // of the step's rows took 4.0: a thread has four pairs or eight rows.
-// AXES: as everywhere, cos / sin of a chunk's own axis.
+// VONLY: V alone (rope_rows_kernel has written K).
 constexpr int KVG_NT = 256;
-template <typename T, bool KV8, bool AXES>
+template <typename T, bool KV8, bool VONLY>
 __global__ __launch_bounds__(KVG_NT) void kv_group_kernel(
     const T* __restrict__ qkv, int64_t qkv_stride, const int64_t* __restrict__ positions,
     const float* __restrict__ cos_sin, void* __restrict__ k_cache, void* __restrict__ v_cache,
     const int64_t* __restrict__ slot_mapping, int T_, int nq, int nkv, int d, int bs, int bs_shift,
-    int num_blocks, float k_inv, float v_inv, int groups, RopeAxes ax) {
+    int num_blocks, float k_inv, float v_inv, int groups) {
   typedef std::conditional_t<KV8, uint8_t, T> C;
   C* kc = reinterpret_cast<C*>(k_cache);
   C* vc = reinterpret_cast<C*>(v_cache);
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(KVG_NT) void kv_group_kernel(
     int64_t sl = slot_mapping[row];
     KGC_DCHECK_RANGE(sl, -1, (int64_t)num_blocks * bs, "KV slot");
     slot = sl < 0 ? -1 : (int)sl;
-    if (!AXES && slot >= 0) pos = (int)positions[row];
+    if (!VONLY && slot >= 0) pos = (int)positions[row];
   }
   const int up = __shfl_down(slot, 1, 64);
   const uint32_t next = (uint32_t)__ballot(slot >= 0 && up == slot + 1 && lane < 21);
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(KVG_NT) void kv_group_kernel(
     off = s - page * bs;
     return (int64_t)page;
   };
-  for (int u = threadIdx.x % tpg; u < (2 * nv + 63 & ~63); u += tpg) {
+  for (int u = threadIdx.x % tpg; u < ((VONLY ? nv : 2 * nv) + 63 & ~63); u += tpg) {
     const int k = max(min(u, 2 * nv - 1) - nv, 0), par = k / (nkv * tph), hc = k - par * (nkv * tph);
     int sl[4], ps[4];                          // (by every lane: a wave can hold units of both kinds)
 #pragma unroll
@@ -272,6 +272,7 @@ __global__ __launch_bounds__(KVG_NT) void kv_group_kernel(
       ps[i] = __shfl(pos, 7 + par + 2 * i, 64);
     }
     if (u >= nv) {                             // ---- K
+      if constexpr (VONLY) continue;
       const int h = hc / tph, c = hc - h * tph;
       Pack8<T> a[4], b[4];
 #pragma unroll
@@ -283,19 +284,12 @@ __global__ __launch_bounds__(KVG_NT) void kv_group_kernel(
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float co[8], si[8];
-        if constexpr (AXES) {
-          axes_cos_sin(ax, positions, min(t0 + par + 2 * i, T_ - 1), cos_sin, d, c * 8, co, si);
-        } else {
-          const float* cs = cos_sin + (int64_t)ps[i] * d + c * 8;
-          const float4 c0 = *reinterpret_cast<const float4*>(cs), c1 = *reinterpret_cast<const float4*>(cs + 4);
-          const float4 s0 = *reinterpret_cast<const float4*>(cs + half);
-          const float4 s1 = *reinterpret_cast<const float4*>(cs + half + 4);
-          co[0] = c0.x; co[1] = c0.y; co[2] = c0.z; co[3] = c0.w;
-          co[4] = c1.x; co[5] = c1.y; co[6] = c1.z; co[7] = c1.w;
-          si[0] = s0.x; si[1] = s0.y; si[2] = s0.z; si[3] = s0.w;
-          si[4] = s1.x; si[5] = s1.y; si[6] = s1.z; si[7] = s1.w;
-        }
+        const float* cs = cos_sin + (int64_t)ps[i] * d + c * 8;
+        const float4 c0 = *reinterpret_cast<const float4*>(cs), c1 = *reinterpret_cast<const float4*>(cs + 4);
+        const float4 s0 = *reinterpret_cast<const float4*>(cs + half);
+        const float4 s1 = *reinterpret_cast<const float4*>(cs + half + 4);
+        const float co[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+        const float si[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
         Pack8<T> oa, ob;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -370,6 +364,61 @@ __global__ __launch_bounds__(KVG_NT) void kv_group_kernel(
   }
 }
 
+// Many tokens with a position per axis: q and K by rows, V by the group kernel above.  A wave has HG neighbouring heads of 8 tokens
+// (16 with heads of 64), a lane the chunk pair (c, c + d / 2) of each, with one load of cos / sin.
+constexpr int ROWS_HG = 4;
+template <typename T, bool KV8>
+__global__ __launch_bounds__(256) void rope_rows_kernel(
+    const T* __restrict__ qkv, int64_t qkv_stride, const int64_t* __restrict__ positions, const float* __restrict__ cos_sin,
+    T* __restrict__ q_out, void* __restrict__ k_cache, const int64_t* __restrict__ slot_mapping, int T_, int nq, int nkv,
+    int d, int bs, float k_inv, int num_blocks, RopeAxes ax) {
+  const int tph = d >> 4, half = d >> 1, heads = nq + nkv, groups = (heads + ROWS_HG - 1) / ROWS_HG, tpw = 64 / tph;
+  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, c = lane % tph, h0 = (int)(wave % groups) * ROWS_HG;
+  const int64_t t = wave / groups * tpw + lane / tph;
+  if (t >= T_) return;
+  const T* src = qkv + t * qkv_stride + c * 8;
+  Pack8<T> a[ROWS_HG], b[ROWS_HG];
+#pragma unroll
+  for (int k = 0; k < ROWS_HG; ++k) {                  // the last group's missing heads: its last one again
+    a[k].u = *reinterpret_cast<const u32x4*>(src + min(h0 + k, heads - 1) * d);
+    b[k].u = *reinterpret_cast<const u32x4*>(src + min(h0 + k, heads - 1) * d + half);
+  }
+  int64_t slot = slot_mapping[t];
+  KGC_DCHECK_RANGE(slot, -1, (int64_t)num_blocks * bs, "KV slot");
+  float cc[8], sn[8];
+  axes_cos_sin(ax, positions, (int)t, cos_sin, d, c * 8, cc, sn);
+#pragma unroll
+  for (int k = 0; k < ROWS_HG; ++k) {
+    const int head = h0 + k;
+    if (head >= heads) break;
+    Pack8<T> oa, ob;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float ra, rb;
+      neox_rot(to_f(a[k].h[j]), to_f(b[k].h[j]), cc[j], sn[j], ra, rb);
+      oa.h[j] = from_f<T>(ra);
+      ob.h[j] = from_f<T>(rb);
+    }
+    if (head < nq) {
+      T* dst = q_out + (t * nq + head) * d + c * 8;
+      *reinterpret_cast<u32x4*>(dst) = oa.u;
+      *reinterpret_cast<u32x4*>(dst + half) = ob.u;
+    } else if (slot >= 0) {
+      const int64_t blk = slot / bs, e = ((blk * nkv + head - nq) * bs + (slot - blk * bs)) * d + c * 8;
+      if constexpr (KV8) {
+        uint8_t* dst = reinterpret_cast<uint8_t*>(k_cache) + e;
+        *reinterpret_cast<u32x2*>(dst) = fp8_8(oa, k_inv);
+        *reinterpret_cast<u32x2*>(dst + half) = fp8_8(ob, k_inv);
+      } else {
+        T* dst = reinterpret_cast<T*>(k_cache) + e;
+        *reinterpret_cast<u32x4*>(dst) = oa.u;
+        *reinterpret_cast<u32x4*>(dst + half) = ob.u;
+      }
+    }
+  }
+}
+
 // KGC_ROPE_KVG=0: prefill K / V writes on the per-token kernel (A/B)
 static bool rope_kvg() {
   const char* e = getenv("KGC_ROPE_KVG");
@@ -403,28 +452,18 @@ static void rope_dispatch(const void* qkv, int64_t qkv_stride, int S, int64_t ss
   const int units = nkv * (d >> 2), groups = units <= 64 ? 4 : units <= 128 ? 2 : 1;      // of one 8-row group
   if (ax.n) {                   // (the host: rotated, q asked for)
     if constexpr (!SL) {
-      // Two launches, q by rows and k / v by 8-row groups, from 4M elements on; us, 32 / 8 heads of 128 in 16-bit pages, one launch ->
-      // two: 500 rows 10.1 -> 11.0, 1000 13.0 -> 12.2, 2000 22.0 -> 17.2, 12000 106.7 -> 72.5; 8 / 1 heads 1000 7.1 -> 8.9,
-      // 4000 14.6 -> 12.6; 1000 of 12 / 12 heads of 64 12.0 -> 12.3.
-      if (!norm && kv_groups() && (d == 64 || d == 128) && (int64_t)T_ * (nq + 2 * nkv) * d >= 4 << 20 &&
+      // Two launches, q and K by rows and V by 8-row groups, from 3M elements on: faster from a third of that on, but the second
+      // launch is 3 us of the host's, who is behind by then.  us in a graph, one launch -> two, 32 / 8 heads of 128 in 16-bit pages: 500
+      // rows 10.1 -> 10.5, 700 11.5 -> 11.2, 1000 13.1 -> 10.8, 2000 22.0 -> 15.1, 12000 106.7 -> 68.5; 8 / 1 heads 1000 7.0 -> 6.6, 2000
+      // 9.1 -> 8.0, 4000 14.6 -> 9.6; 12 / 12 heads of 64 300 8.1 -> 8.9, 1000 12.0 -> 9.1.
+      if (!norm && kv_groups() && (d == 64 || d == 128) && (int64_t)T_ * (nq + 2 * nkv) * d >= 3 << 20 &&
           reinterpret_cast<uintptr_t>(qkv) % 16 == 0 && reinterpret_cast<uintptr_t>(q_out) % 16 == 0) {
-        Kv4Write w{};           // q alone: no kv heads
-        w.qkv = qkv;
-        w.qkv_stride = qkv_stride;
-        w.positions = pos;
-        w.cos_sin = cs;
-        w.q_out = q_out;
-        w.slots = slots;
-        w.T = T_;
-        w.nq = nq;
-        w.d = d;
-        w.bs = bs;
-        w.num_blocks = num_blocks;
-        w.use_rope = true;
-        launch_kv4_write(std::is_same_v<T, bf16> ? DT_BF16 : DT_F16, w, ax, s);
+        const int64_t waves = ((int64_t)T_ * (d >> 4) + 63) / 64 * ((nq + nkv + ROWS_HG - 1) / ROWS_HG);
+        rope_rows_kernel<T, KV8><<<(unsigned)((waves + 3) / 4), 256, 0, s>>>(
+            (const T*)qkv, qkv_stride, pos, cs, (T*)q_out, kc, slots, T_, nq, nkv, d, bs, k_inv, num_blocks, ax);
         kv_group_kernel<T, KV8, true><<<(T_ + 8 * groups - 1) / (8 * groups), KVG_NT, 0, s>>>(
             (const T*)qkv, qkv_stride, pos, cs, kc, vc, slots, T_, nq, nkv, d, bs,
-            (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1, num_blocks, k_inv, v_inv, groups, ax);
+            (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1, num_blocks, k_inv, v_inv, groups);
         return;
       }
     }
@@ -436,7 +475,7 @@ static void rope_dispatch(const void* qkv, int64_t qkv_stride, int S, int64_t ss
     if (kvo && rope && !norm && rope_kvg() && kv_groups()) {
       kv_group_kernel<T, KV8, false><<<(T_ + 8 * groups - 1) / (8 * groups), KVG_NT, 0, s>>>(
           (const T*)qkv, qkv_stride, pos, cs, kc, vc, slots, T_, nq, nkv, d, bs,
-          (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1, num_blocks, k_inv, v_inv, groups, ax);
+          (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1, num_blocks, k_inv, v_inv, groups);
       return;
     }
   }

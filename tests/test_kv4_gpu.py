@@ -132,7 +132,7 @@ def test_write_with_norms(gpu, cache, sections):
 @pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("cache", ["auto", "fp8"])
 @pytest.mark.parametrize("T,sections,slices", [(77, (16, 24, 24), 0), (77, (5, 0, 40, 19), 0), (9, (64,), 2), (700, (16, 24, 24), 0),
-                                               (521, (60, 1, 3), 0)])
+                                               (521, (60, 1, 3), 0), (2851, (16, 24, 24), 0), (2400, (3, 50, 11), 0)])
 def test_axes_of_the_wider_caches(gpu, dt, cache, T, sections, slices):
     g, nq, nkv, d, bs = _gen(7), 8, 2, 128, 16
     t = torch.float8_e4m3fn if cache == "fp8" else dt
