@@ -246,7 +246,6 @@ __global__ __launch_bounds__(256, BUFS == 2 ? 2 : D == 128 ? 3 : 4) void kv4_pre
 }
 
 // D / 4 threads per row of a work item's block and head, four elements each; slices' partials eight at a time.
-constexpr int KV4_MAX_SLICES = 32;
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(
     T* __restrict__ out, const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ qsl,

@@ -251,6 +251,10 @@ PROMPTS = [
     (16, 1, 128, 16, [33, 90], [31, 1]),
     (7, 1, 64, 32, [300], [0]),
     (1, 1, 128, 32, [1, 1, 1], [0, 64, 255]),
+    # many items
+    (32, 8, 128, 32, [1 + 17 * i % 150 for i in range(60)], [5 * i % 90 for i in range(60)]),
+    (12, 12, 64, 16, [2 + 11 * i % 130 for i in range(100)], [7 * i % 40 for i in range(100)]),
+    (12, 6, 128, 64, [3 + 29 * i % 140 for i in range(70)], [0] * 70),
 ]
 
 
