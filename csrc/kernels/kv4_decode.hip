@@ -143,14 +143,18 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_decode_kernel(
         }
     }
     m = kv4_max_rows(m);
-    // a row none of whose scores is above -inf (q or k too large): no difference of infinities
-    const float ref = m == -INFINITY ? 0.f : m;
-    const float alpha = __builtin_amdgcn_exp2f(m_run - ref);
-    m_run = m;
-    l_run *= alpha;
+    // The reference moves only where the maximum is more than 2^8 above it: probabilities are then at most 2^8, and O is seldom
+    // rescaled.
+    if (__any(m > m_run + 8.f)) {
+      const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m);
+      m_run = m;
+      l_run *= f;
 #pragma unroll
-    for (int t = 0; t < DT; ++t) o[t] *= alpha;
-    // probabilities are at most 1 and rounded to T for the product, as the keys' and values' type has it; their sum is not
+      for (int t = 0; t < DT; ++t) o[t] *= f;
+    }
+    // a row none of whose scores is above -inf (q or k too large): no difference of infinities
+    const float ref = m_run == -INFINITY ? 0.f : m_run;
+    // probabilities are rounded to T for the product, as the keys' and values' type has it; their sum is not
     Pack8<T> pf;
 #pragma unroll
     for (int g = 0; g < 2; ++g)
