@@ -259,6 +259,7 @@ static void kv4_decode_dispatch(const Kv4Decode& a, int waves, DecodeLeast least
       a.ctx_lens, a.max_logits, a.exp_sums, a.tmp_out, a.nq, a.nkv, a.bs_log2, sl2, a.num_blocks, least)
   if (waves == 8) KGC_KV4_DEC(8);
   else if (waves == 4) KGC_KV4_DEC(4);
+  else if (waves == 2) KGC_KV4_DEC(2);
   else KGC_KV4_DEC(1);
 #undef KGC_KV4_DEC
 }
@@ -270,9 +271,10 @@ static void kv4_decode_dispatch(const Kv4Decode& a, int waves, DecodeLeast least
 //   up to 512 eight waves take the place of slices: 32 x 2000 16.5 (four 20.5, four and two slices -> 21.1), 33 x 1001 of 12 heads of
 //     64 10.5 (10.8, -> 13.5);
 //   from 512 on the LDS of eight (two workgroups per CU) makes short contexts wait: 64 x 512 10.8 (11.3), 64 x 8192 96.6 (97.2);
-//   from 1024 on a wave has a pair to itself: 256 x 60 8.1 (four 13.1, eight 20.5), 128 x 1000 30.6 (31.6, 32.0), 256 x 640 36.3
-//     (39.0, 47.1); long ones are slower so, 128 x 4000 104 (four 108, eight 95).
-static int kv4_decode_waves(int64_t pairs) { return pairs >= 1024 ? 1 : pairs >= 512 ? 4 : pairs >= 64 ? 8 : 4; }
+//   from 1024 on two, 100 x 1000 of 12 heads of 64 24.8 (one 28.6), 128 x 1000 31.0 (34.3, four 31.6);
+//   from 1536 on a wave has a pair to itself: 256 x 60 8.1 (two 11.0, four 13.1), 256 x 640 36.3 (36.7, 39.0), 200 x 1000 47.6
+//     (48.8).
+static int kv4_decode_waves(int64_t pairs) { return pairs >= 1536 ? 1 : pairs >= 1024 ? 2 : pairs >= 512 ? 4 : pairs >= 64 ? 8 : 4; }
 
 void launch_kv4_decode(int dtype, const Kv4Decode& a, float scale, hipStream_t s) {
   if (a.B == 0) return;

@@ -250,7 +250,7 @@ KV4_TARGET_WAVES = 2048      # 4-bit decode: 8 resident waves per CU
 
 def kv4_decode_waves(pairs: int) -> int:
     """Waves that share a slice (csrc/kernels/kv4_decode.hip kv4_decode_waves)."""
-    return 1 if pairs >= 1024 else 4 if pairs >= 512 else 8 if pairs >= 64 else 4
+    return 1 if pairs >= 1536 else 2 if pairs >= 1024 else 4 if pairs >= 512 else 8 if pairs >= 64 else 4
 
 
 def decode_grid_z(batch: int, num_kv_heads: int, max_ctx: int, target_waves: int = 0,

@@ -208,6 +208,7 @@ DECODE = [
     (8, 8, 64, 32, [2100, 1, 0, 90, 64, 33, 500, 2, 7]),
     (8, 8, 64, 16, [1 + 7 * i % 67 for i in range(70)]),
     (8, 8, 64, 32, [3 * i % 71 for i in range(130)]),
+    (4, 4, 64, 32, [5 * i % 77 for i in range(400)]),
 ]
 
 
