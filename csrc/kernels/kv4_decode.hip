@@ -271,9 +271,10 @@ static void kv4_decode_dispatch(const Kv4Decode& a, int waves, DecodeLeast least
 //   up to 512 eight waves take the place of slices: 32 x 2000 16.5 (four 20.5, four and two slices -> 21.1), 33 x 1001 of 12 heads of
 //     64 10.5 (10.8, -> 13.5);
 //   from 512 on the LDS of eight (two workgroups per CU) makes short contexts wait: 64 x 512 10.8 (11.3), 64 x 8192 96.6 (97.2);
-//   from 1024 on two, 100 x 1000 of 12 heads of 64 24.8 (one 28.6), 128 x 1000 31.0 (34.3, four 31.6);
-//   from 1536 on a wave has a pair to itself: 256 x 60 8.1 (two 11.0, four 13.1), 256 x 640 36.3 (36.7, 39.0), 200 x 1000 47.6
-//     (48.8).
+//   from 1024 on two: 128 x 1000 27.6 (one 31.1, four 27.9), 160 x 1000 34.0 (36.9, 36.1), 128 x 4000 94.1 (99.9, 96.0), 100 x 1000 of
+//     12 heads of 64 22.5 (27.2, 22.9), 128 x 300 12.8 (12.8, 13.6); a short context pays for it, 128 x 60 7.8 (6.1, 8.0);
+//   from 1536 on a wave has a pair to itself: 256 x 60 8.0 (two 10.7, four 13.4), 256 x 640 34.0 (35.0, 38.8), 200 x 1000 42.7
+//     (43.4, 43.3), 250 x 500 of 12 heads of 64 25.4 (28.6, 30.9), 130 x 1000 of them 28.9 (28.9, 29.9).
 static int kv4_decode_waves(int64_t pairs) { return pairs >= 1536 ? 1 : pairs >= 1024 ? 2 : pairs >= 512 ? 4 : pairs >= 64 ? 8 : 4; }
 
 void launch_kv4_decode(int dtype, const Kv4Decode& a, float scale, hipStream_t s) {
