@@ -131,6 +131,7 @@ void check_kv4(const Tensor& k_cache, const Tensor& v_cache, int64_t nkv, int64_
   TORCH_CHECK(k_cache.scalar_type() == at::kByte && v_cache.scalar_type() == at::kByte,
               "k/v cache dtype mismatch: a 4-bit cache is uint8, keys and values");
   TORCH_CHECK(d == 64 || d == 128, "4-bit cache: head_dim must be 64 or 128");
+  TORCH_CHECK(nkv >= 1, "4-bit cache: no heads");
   TORCH_CHECK(k_cache.dim() == 4 && v_cache.dim() == 4 && k_cache.is_contiguous() && v_cache.is_contiguous() &&
               k_cache.sizes() == v_cache.sizes() && k_cache.size(1) == nkv && k_cache.size(3) == d / 2 + d / 32,
               "4-bit cache: k_cache and v_cache uint8 [nb, ", nkv, ", bs, ", d / 2 + d / 32, "] contiguous");

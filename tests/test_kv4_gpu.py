@@ -555,3 +555,14 @@ def test_refusals(gpu):
     no("slots int64", ops.kv4_read, kc, pos.int(), bf)
     no("bf16 / fp16", ops.kv4_read, kc, pos, torch.float32)
     no("4-bit cache", ops.kv4_read, kc[..., :60].contiguous(), pos, bf)
+
+
+def test_a_cache_without_heads_is_refused(gpu):
+    d = 128
+    kc = torch.zeros(ops.kv4_cache_shape(4, 1, 16, d), dtype=torch.uint8, device=gpu)[:, :0].contiguous()
+    pos = torch.zeros(3, dtype=torch.int64, device=gpu)
+    with pytest.raises(RuntimeError, match="no heads"):
+        ops.kv4_read(kc, pos, torch.bfloat16)
+    with pytest.raises(RuntimeError, match="no heads"):
+        ops.rope_kv_write(torch.zeros(3, 4 * d, dtype=torch.bfloat16, device=gpu), pos, torch.zeros(8, d, device=gpu),
+                          kc, kc.clone(), pos, 4, 0, d)
