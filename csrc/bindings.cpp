@@ -221,7 +221,7 @@ void check_kv4_attention(const Tensor& q, const Tensor& out, const Tensor& k_cac
   const int64_t nq = q.size(1), nkv = k_cache.size(1);
   check_kv4(k_cache, v_cache, nkv, q.size(2), q);
   no_kv4_scale(k_scale, v_scale);
-  TORCH_CHECK(nq % nkv == 0 && nq / nkv <= 16, "GQA group must be <= 16");
+  TORCH_CHECK(nq >= 1 && nq % nkv == 0 && nq / nkv <= 16, "GQA group must be 1 to 16 heads");
   TORCH_CHECK(k_cache.size(0) >= 1 || q.size(0) == 0, "4-bit cache: no pages");
   TORCH_CHECK(q.size(0) < ((int64_t)1 << 31), "rows");
   TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out");

@@ -394,7 +394,7 @@ def kv4_prefill_slices(rows: int, seqs: int, num_heads: int, num_kv_heads: int, 
     tiles = math.ceil(max_len / 64)
     if tiles < 12:
         return 1
-    g = num_heads // num_kv_heads
+    g = num_heads // max(num_kv_heads, 1)                     # (no heads: the op refuses them)
     heads = 4 if g % 4 == 0 else 2 if g % 2 == 0 else 1
     blocks = seqs * math.ceil(rows / max(seqs, 1) * heads / PREFILL_BLOCK_M) * (num_heads // heads)
     return max(1, min((512 if head_dim == 128 else 768) // max(blocks, 1), tiles // 4, 16))

@@ -178,3 +178,8 @@ def test_decode_slices_of_a_4bit_cache():
                 assert 1 <= z <= 1024 and (z == 1 or (z - 1) * 64 < ctx)
                 ws = ops.decode_partials(B, nkv, 64, -(-ctx // 32), 32, "meta")
                 assert z <= ws[0].numel() // (B * nkv), (B, nkv, ctx, z)
+
+
+def test_slices_of_prompts_without_heads():
+    """Shapes that the op refuses get there: the host's rule does not divide by their heads."""
+    assert ops.kv4_prefill_slices(5, 1, 4, 0, 64, 5000) >= 1 and ops.kv4_prefill_slices(5, 1, 0, 0, 64, 5000) >= 1

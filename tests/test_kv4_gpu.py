@@ -566,3 +566,17 @@ def test_a_cache_without_heads_is_refused(gpu):
     with pytest.raises(RuntimeError, match="no heads"):
         ops.rope_kv_write(torch.zeros(3, 4 * d, dtype=torch.bfloat16, device=gpu), pos, torch.zeros(8, d, device=gpu),
                           kc, kc.clone(), pos, 4, 0, d)
+
+
+@pytest.mark.parametrize("nq,nkv", [(0, 2), (4, 0), (0, 0)])
+def test_queries_without_heads_are_refused(gpu, nq, nkv):
+    d = 128
+    kc = torch.zeros(ops.kv4_cache_shape(4, max(nkv, 1), 16, d), dtype=torch.uint8, device=gpu)[:, :nkv].contiguous()
+    q = torch.zeros(3, nq, d, dtype=torch.bfloat16, device=gpu)
+    bt = torch.zeros(3, 64, dtype=torch.int32, device=gpu)
+    n = torch.ones(3, dtype=torch.int32, device=gpu)
+    for z in (1, 2):
+        with pytest.raises(RuntimeError, match="GQA group|4-bit cache"):
+            ops.paged_attention_decode(q, kc, kc, bt, n, 1.0, None, z)
+    with pytest.raises(RuntimeError, match="GQA group|4-bit cache"):
+        ops.prefill_attention(q, kc, kc, bt, torch.arange(4, dtype=torch.int32, device=gpu), n, 1.0)
