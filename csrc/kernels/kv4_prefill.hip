@@ -58,12 +58,14 @@ __global__ __launch_bounds__(256, BUFS == 2 ? 2 : D == 128 ? 3 : 4) void kv4_pre
   const int seq = work_seq[item], mb = work_mblk[item];
   const int h = group / (G / GH), head0 = h * G + group % (G / GH) * GH;
   if (seq < 0 || seq >= seqs || mb < 0) return;        // the whole workgroup, and so below
-  const int q0 = qsl[seq], qlen = qsl[seq + 1] - q0;
+  const int q0 = qsl[seq], q1 = qsl[seq + 1];
   int L_in = seq_lens[seq];
   KGC_DCHECK_RANGE(L_in, 0, (bt_stride << bs_log2) + 1, "prefill seq_len");
-  const int L = min(L_in, bt_stride << bs_log2), ctx0 = L - qlen;
-  const int qbase = mb * KV4_BM + sub * QB;
-  if (q0 < 0 || qlen <= 0 || qlen > rows_all - q0 || ctx0 < 0 || qbase >= qlen) return;
+  const int L = min(L_in, bt_stride << bs_log2);
+  // (compared before they are subtracted or multiplied: no difference or product of numbers that are none wraps)
+  if (q0 < 0 || q1 <= q0 || q1 > rows_all || L < q1 - q0 || mb > (q1 - q0 - 1) / KV4_BM) return;
+  const int qlen = q1 - q0, ctx0 = L - qlen, qbase = mb * KV4_BM + sub * QB;
+  if (qbase >= qlen) return;
   const int* bt = block_tables + (int64_t)seq * bt_stride;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 31, hi = lane >> 5;
   const int bs = 1 << bs_log2, bsm = bs - 1;
@@ -255,9 +257,10 @@ __global__ __launch_bounds__(256) void kv4_prefill_merge_kernel(
   const int item = blockIdx.x / nq, head = blockIdx.x % nq;
   const int seq = work_seq[item], mb = work_mblk[item];
   if (seq < 0 || seq >= seqs || mb < 0) return;
-  const int q0 = qsl[seq], qlen = qsl[seq + 1] - q0;
+  const int q0 = qsl[seq], q1 = qsl[seq + 1];
+  if (q0 < 0 || q1 <= q0 || q1 > rows_all || min(seq_lens[seq], cap) < q1 - q0 || mb > (q1 - q0 - 1) / KV4_BM) return;
   const int r = mb * KV4_BM + blockIdx.y * ROWS + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-  if (q0 < 0 || qlen > rows_all - q0 || r >= qlen || min(seq_lens[seq], cap) < qlen) return;    // as the kernel above
+  if (r >= q1 - q0) return;                              // as the kernel above
   const int64_t row = ((int64_t)(q0 + r) * nq + head) * Z;
   float top = -INFINITY, total = 0.f;
   for (int z = 0; z < Z; ++z) top = fmaxf(top, part_ml[2 * (row + z)]);

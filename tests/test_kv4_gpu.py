@@ -580,3 +580,32 @@ def test_queries_without_heads_are_refused(gpu, nq, nkv):
             ops.paged_attention_decode(q, kc, kc, bt, n, 1.0, None, z)
     with pytest.raises(RuntimeError, match="GQA group|4-bit cache"):
         ops.prefill_attention(q, kc, kc, bt, torch.arange(4, dtype=torch.int32, device=gpu), n, 1.0)
+
+
+@pytest.mark.parametrize("z", [1, 4])
+def test_numbers_that_would_wrap(gpu, z):
+    """Work items, row ranges and lengths whose products or differences leave 32 bits are left out like others that
+    are none: 2^24 blocks of 128 rows are -2^31, 2^25 are 0."""
+    if ops.DEBUG:
+        pytest.skip("the bounds-checking build reports them")
+    low = -2 ** 31
+    new, old = [20, 40], [100, 300]
+    q, kc, vc, bt, totals = _attention_case(9, 4, 2, 64, 32, torch.bfloat16, new, old)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=gpu)   # noqa: E731
+    qg, a = q.to(gpu), [t.to(gpu) for t in (kc, vc, bt)]
+    parts = torch.empty(z * q.numel() // 64 * 66, device=gpu)
+
+    def run(starts, n, ws, wm):
+        out = torch.full_like(qg, 7)
+        torch.ops.kgc.prefill_attention(out, qg, *a, starts, n, ws, wm, 0.125, 1.0, 1.0, 0, parts)
+        return out
+    # (the second sequence's only true item comes first; items of block 0, again, would write the same rows)
+    out = run(_starts(new).to(gpu), i32(*totals), i32(1, 0, 0, 0, 0), i32(0, 1 << 24, 1 << 25, 2 ** 31 - 1, (1 << 24) + 1))
+    assert (out[:20] == 7).all()
+    _check_attention(out[20:].cpu(), q[20:], kc, vc, bt[1:], new[1:], totals[1:], 0.125)
+    for starts, n in ((i32(low, low + 20, 60), i32(*totals)), (i32(5, low, low + 3), i32(*totals)), (i32(0, 2 ** 31 - 1, 60), i32(*totals)),
+                      (_starts(new).to(gpu), i32(low, low + 7))):
+        assert (run(starts, n, i32(0, 1), i32(0, 0)) == 7).all()
+    dec = ops.paged_attention_decode(torch.stack([q[0], q[59]]).to(gpu), *a, i32(low, totals[1]), 0.125, None, z)
+    assert not dec[0].any()
+    _check_attention(dec[1:].cpu(), q[59:], kc, vc, bt[1:], [1], totals[1:], 0.125)
