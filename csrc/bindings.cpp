@@ -126,6 +126,7 @@ kgc::RopeAxes rope_axes(const Tensor& positions, at::OptionalIntArrayRef section
   return ax;
 }
 
+constexpr int64_t GRID_THREADS = (int64_t)1 << 32;     // of a launch, in x: fewer than these
 // ---- the cache in 4 bits: uint8 [nb, nkv, bs, d / 2 + d / 32], a head's page as csrc/kernels/kv4.h has it
 void check_kv4(const Tensor& k_cache, const Tensor& v_cache, int64_t nkv, int64_t d, const Tensor& with) {
   TORCH_CHECK(k_cache.scalar_type() == at::kByte && v_cache.scalar_type() == at::kByte,
@@ -159,7 +160,7 @@ void kv4_write(const Tensor& qkv, int64_t stride, int64_t S, int64_t slice_strid
   no_kv4_scale(k_scale, v_scale);
   TORCH_CHECK(!use_rope || ax.rows > 0, "kgc.rope_kv_write: an empty cos_sin");
   TORCH_CHECK(slot_mapping.is_contiguous() && (ax.n || positions.is_contiguous()), "positions, slot_mapping contiguous");
-  TORCH_CHECK(T * (nq + 2 * nkv) * (d / 16) < ((int64_t)1 << 31) * 256 && T < ((int64_t)1 << 31), "kgc.rope_kv_write: rows");
+  TORCH_CHECK(T * (nq + 2 * nkv) * (d / 16) < GRID_THREADS - (1 << 24) && T < ((int64_t)1 << 31), "kgc.rope_kv_write: rows");
   aligned16(qkv, "qkv");
   aligned16(q_out, "q_out");
   aligned16(cos_sin, "cos_sin");
@@ -205,7 +206,7 @@ Tensor kv4_read(Tensor cache, Tensor slots, at::ScalarType dtype) {
   check_kv4(cache, cache, nkv, d, cache);
   TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous(), "kgc.kv4_read: slots int64 [n]");
   check_same_dev(cache, slots, "slots");
-  TORCH_CHECK(slots.numel() * nkv * (d / 8) < ((int64_t)1 << 31) * 256, "kgc.kv4_read: rows");
+  TORCH_CHECK(slots.numel() * nkv * (d / 8) < 4 * (GRID_THREADS - (1 << 24)), "kgc.kv4_read: rows");    // four a thread
   Tensor out = at::empty({slots.numel(), nkv, d}, cache.options().dtype(dtype));
   if (cache.size(0) == 0) out.zero_();
   kgc::launch_kv4_read(dt_code(out), out.data_ptr(), cache.data_ptr(), slots.data_ptr<int64_t>(), out.size(0), (int)nkv,
@@ -227,8 +228,8 @@ void check_kv4_attention(const Tensor& q, const Tensor& out, const Tensor& k_cac
   TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), "out");
   check_same_dev(q, out, "out");
   TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.is_contiguous() &&
-              block_tables.size(1) >= 1 && block_tables.size(1) * k_cache.size(2) < ((int64_t)1 << 31),
-              "block_tables int32 [rows, max_blocks] contiguous");
+              block_tables.size(1) >= 1 && block_tables.size(1) * k_cache.size(2) <= ((int64_t)1 << 30),
+              "block_tables int32 [rows, max_blocks] contiguous, of 2^30 tokens a row or fewer");
   check_same_dev(q, block_tables, "block_tables");
   aligned16(q, "q");
   aligned16(out, "out");
@@ -336,7 +337,7 @@ void kv4_decode_into(const Tensor& out, const Tensor& q, const Tensor& k_cache, 
                      double v_scale) {
   check_kv4_attention(q, out, k_cache, v_cache, block_tables, k_scale, v_scale);
   const int64_t B = q.size(0), nq = q.size(1), d = q.size(2);
-  TORCH_CHECK(B < ((int64_t)1 << 31) && k_cache.size(1) <= 65535 && nq <= 65535, "grid");
+  TORCH_CHECK(B * 64 < GRID_THREADS && k_cache.size(1) <= 65535 && nq <= 65535, "kgc.paged_decode: too many rows or heads for a launch");
   TORCH_CHECK(block_tables.size(0) >= B, "block_tables int32 [B, max_blocks]");
   TORCH_CHECK(ctx_lens.scalar_type() == at::kInt && ctx_lens.is_contiguous() && ctx_lens.numel() >= B, "ctx_lens int32 [B]");
   check_same_dev(q, ctx_lens, "ctx_lens");
@@ -499,7 +500,6 @@ void kv4_prefill_into(const Tensor& out, const Tensor& q, const Tensor& k_cache,
   TORCH_CHECK(work_seq.scalar_type() == at::kInt && work_mblk.scalar_type() == at::kInt && work_seq.is_contiguous() &&
               work_mblk.is_contiguous() && work_seq.numel() == work_mblk.numel(), "work list");
   for (const Tensor* t : {&query_start_loc, &seq_lens, &work_seq, &work_mblk}) check_same_dev(q, *t, "prefill operand");
-  TORCH_CHECK(work_seq.numel() <= 2147483647 && q.size(1) <= 65535, "grid");
   kgc::Kv4Prefill a{};
   a.Z = 1;
   if (partials.has_value()) {
@@ -512,7 +512,7 @@ void kv4_prefill_into(const Tensor& out, const Tensor& q, const Tensor& k_cache,
     a.part_o = partials->data_ptr<float>();
     a.part_ml = a.part_o + rows * a.Z * q.size(2);
   }
-  TORCH_CHECK(work_seq.numel() * q.size(1) * a.Z < ((int64_t)1 << 31), "grid");
+  TORCH_CHECK(work_seq.numel() * q.size(1) * a.Z < GRID_THREADS / 256, "kgc.prefill_attention: too many work items for a launch");
   a.q = q.data_ptr();
   a.k_cache = k_cache.data_ptr();
   a.v_cache = v_cache.data_ptr();

@@ -609,3 +609,21 @@ def test_numbers_that_would_wrap(gpu, z):
     dec = ops.paged_attention_decode(torch.stack([q[0], q[59]]).to(gpu), *a, i32(low, totals[1]), 0.125, None, z)
     assert not dec[0].any()
     _check_attention(dec[1:].cpu(), q[59:], kc, vc, bt[1:], [1], totals[1:], 0.125)
+
+
+def test_launches_up_to_their_limit(gpu):
+    """2^24 workgroups of 256 prompt threads are more than a launch takes: refused; the longest list below them runs."""
+    new, old, nq = [20], [100], 16
+    q, kc, vc, bt, totals = _attention_case(9, nq, 1, 64, 32, torch.bfloat16, new, old)
+    a = [t.to(gpu) for t in (q, kc, vc, bt, _starts(new), torch.tensor(totals, dtype=torch.int32))]
+    items = (1 << 24) // nq
+    ws, wm = torch.full((items,), -1, dtype=torch.int32, device=gpu), torch.zeros(items, dtype=torch.int32, device=gpu)
+    with pytest.raises(RuntimeError, match="too many work items"):
+        ops.prefill_attention(*a, 0.125, ws, wm)
+    ws[-2] = 0
+    out = torch.full_like(a[0], 7)
+    ops.prefill_attention(*a, 0.125, ws[:-1], wm[:-1], out=out)
+    _check_attention(out.cpu(), q, kc, vc, bt, new, totals, 0.125)
+    wide = torch.zeros(1, (1 << 25) + 1, dtype=torch.int32, device=gpu)
+    with pytest.raises(RuntimeError, match="2\\^30"):
+        ops.paged_attention_decode(a[0][:1], *a[1:3], wide, a[5], 0.125)
