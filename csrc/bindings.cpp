@@ -6,6 +6,7 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <cmath>
 
 #include "kernels/chunk_rows.h"
 #include "kernels/launch.h"
@@ -493,6 +494,7 @@ void kv4_prefill_into(const Tensor& out, const Tensor& q, const Tensor& k_cache,
                       const Tensor& work_seq, const Tensor& work_mblk, double scale, double k_scale, double v_scale,
                       const std::optional<Tensor>& partials) {
   check_kv4_attention(q, out, k_cache, v_cache, block_tables, k_scale, v_scale);
+  TORCH_CHECK((float)scale > 0.f && std::isfinite((float)scale), "kgc.prefill_attention: a 4-bit cache's prompts take a scale above zero");
   const int64_t P = block_tables.size(0);
   TORCH_CHECK(query_start_loc.scalar_type() == at::kInt && query_start_loc.is_contiguous() &&
               query_start_loc.numel() == P + 1, "query_start_loc");

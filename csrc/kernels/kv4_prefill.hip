@@ -159,6 +159,7 @@ __global__ __launch_bounds__(256, BUFS == 2 ? 2 : D == 128 ? 3 : 4) void kv4_pre
           for (int i = 0; i < 16; ++i)
             if (key0 + 32 * g + 8 * (i >> 2) + (i & 3) > qpos) s[g][i] = -INFINITY;
       }
+      // scores are scaled behind their maximum and their mask: the scale is above zero (the host refuses others)
       float top = s[0][0];
 #pragma unroll
       for (int g = 0; g < 2; ++g)

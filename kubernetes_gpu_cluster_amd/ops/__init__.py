@@ -407,7 +407,7 @@ def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
                       out: Optional[torch.Tensor] = None, k_scale: float = 1.0,
                       v_scale: float = 1.0, max_len: int = 0) -> torch.Tensor:
     """``max_len``: no sequence is longer (0: not known; the tables' width is taken for it).  It
-    chooses between kernels, and limits nothing."""
+    chooses between kernels, and limits nothing.  ``scale`` is above zero."""
     if not _gpu(q):
         return ref.prefill_attention(q, k_cache, v_cache, block_tables, query_start_loc,
                                      seq_lens, scale, k_scale, v_scale)

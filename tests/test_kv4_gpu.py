@@ -627,3 +627,20 @@ def test_launches_up_to_their_limit(gpu):
     wide = torch.zeros(1, (1 << 25) + 1, dtype=torch.int32, device=gpu)
     with pytest.raises(RuntimeError, match="2\\^30"):
         ops.paged_attention_decode(a[0][:1], *a[1:3], wide, a[5], 0.125)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), float("inf"), 1e-60, 1e60])
+def test_scales_of_prompts(gpu, scale):
+    """The prompt kernel scales behind the mask and the maximum: a scale that is not above zero, in 32 bits, is refused.
+    Decode scales first and takes those that are numbers."""
+    new, old = [40, 1], [30, 70]
+    q, kc, vc, bt, totals = _attention_case(3, 4, 2, 64, 32, torch.bfloat16, new, old)
+    a = [t.to(gpu) for t in (q, kc, vc, bt, _starts(new), torch.tensor(totals, dtype=torch.int32))]
+    with pytest.raises(RuntimeError, match="above zero"):
+        ops.prefill_attention(*a, scale)
+    with pytest.raises(RuntimeError, match="above zero"):
+        ops.prefill_attention(*a, scale, out=torch.empty_like(a[0]))
+    if abs(scale) < 1:
+        last = q[[39, 40]]
+        got = ops.paged_attention_decode(last.to(gpu), *a[1:4], a[5], scale)
+        _check_attention(got.cpu(), last, kc, vc, bt, [1, 1], totals, scale)
