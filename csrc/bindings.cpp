@@ -160,19 +160,12 @@ void kv4_write(const Tensor& qkv, int64_t stride, int64_t S, int64_t slice_strid
   check_kv4(k_cache, v_cache, nkv, d, qkv);
   no_kv4_scale(k_scale, v_scale);
   TORCH_CHECK(!use_rope || ax.rows > 0, "kgc.rope_kv_write: an empty cos_sin");
-  TORCH_CHECK(slot_mapping.is_contiguous() && (ax.n || positions.is_contiguous()), "positions, slot_mapping contiguous");
   TORCH_CHECK(T * (nq + 2 * nkv) * (d / 16) < GRID_THREADS - (1 << 24) && T < ((int64_t)1 << 31), "kgc.rope_kv_write: rows");
   aligned16(qkv, "qkv");
   aligned16(q_out, "q_out");
   aligned16(cos_sin, "cos_sin");
   kgc::Kv4Write w{};
   if (q_norm_w.has_value()) {
-    TORCH_CHECK(k_norm_w.has_value() && q_norm_w->numel() == d && k_norm_w->numel() == d, "qk norm weights");
-    for (const Tensor* t : {&*q_norm_w, &*k_norm_w}) {
-      TORCH_CHECK(t->scalar_type() == q_out.scalar_type() && t->is_contiguous(), "qk norm weights in q's dtype");
-      check_same_dev(qkv, *t, "qk norm weights");
-      aligned16(*t, "qk norm weights");
-    }
     w.q_norm_w = q_norm_w->data_ptr();
     w.k_norm_w = k_norm_w->data_ptr();
   }
@@ -269,8 +262,17 @@ void rope_kv_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor q_out, T
               "q_out bf16 / fp16");
   const kgc::RopeAxes ax = rope_axes(positions, sections, cos_sin, T, d, use_rope);
   TORCH_CHECK(slot_mapping.scalar_type() == at::kLong && slot_mapping.numel() == T, "slot_mapping int64 [T]");
+  TORCH_CHECK(slot_mapping.is_contiguous() && (ax.n || positions.is_contiguous()), "positions, slot_mapping contiguous");
   TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() && cos_sin.size(1) == d,
               "cos_sin fp32 [max_pos, d]");
+  if ((kv4 || ax.n) && q_norm_w.has_value()) {
+    TORCH_CHECK(k_norm_w.has_value() && q_norm_w->numel() == d && k_norm_w->numel() == d, "qk norm weights");
+    for (const Tensor* t : {&*q_norm_w, &*k_norm_w}) {
+      TORCH_CHECK(t->scalar_type() == q_out.scalar_type() && t->is_contiguous(), "qk norm weights in q's dtype");
+      check_same_dev(qkv, *t, "qk norm weights");
+      aligned16(*t, "qk norm weights");
+    }
+  }
   // an empty q_out: write k / v only (prefill_attention_rope rotates q as it loads it)
   const bool kv_only = q_out.numel() == 0;
   TORCH_CHECK(kv_only || (q_out.is_contiguous() && q_out.numel() == T * nq * d),

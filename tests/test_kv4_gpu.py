@@ -644,3 +644,32 @@ def test_scales_of_prompts(gpu, scale):
         last = q[[39, 40]]
         got = ops.paged_attention_decode(last.to(gpu), *a[1:4], a[5], scale)
         _check_attention(got.cpu(), last, kc, vc, bt, [1, 1], totals, scale)
+
+
+@pytest.mark.parametrize("cache", ["auto", "fp8", "fp4"])
+def test_axes_refuse_strides_and_norms_of_other_kinds(gpu, cache):
+    """Slots are read one after the other, norm weights as numbers of q's type on its device, whatever the pages hold."""
+    d, T, bf = 64, 8, torch.bfloat16
+    if cache == "fp4":
+        kc, vc = (torch.zeros(ops.kv4_cache_shape(2, 1, 16, d), dtype=torch.uint8, device=gpu) for _ in range(2))
+    else:
+        t = torch.float8_e4m3fn if cache == "fp8" else bf
+        kc, vc = torch.zeros(2, 1, 16, d, device=gpu).to(t), torch.zeros(2, 1, 2, d, 8, device=gpu).to(t)
+    x = torch.randn(T, 4 * d, device=gpu).to(bf)
+    table = ref.rope_cos_sin_cache(d, 20, 10000.0).to(gpu)
+    slots = torch.arange(2 * T, device=gpu)
+    pos, w = torch.zeros(2, T, dtype=torch.int64, device=gpu), torch.ones(d, dtype=bf, device=gpu)
+
+    def write(slots, *norms, pos=pos, sections=(16, 16)):
+        return ops.rope_kv_write(x, pos, table, kc, vc, slots, 2, 1, d, *norms, sections=sections)
+    for bad in ((slots[::2],), (slots[:T], w.cpu(), w), (slots[:T], w, w.float()), (slots[:T], w, w[:8]), (slots[:T], w, None),
+                (slots[:T], torch.ones(2 * d, dtype=bf, device=gpu)[::2], w)):
+        with pytest.raises(RuntimeError, match="contiguous|norm weights"):
+            write(*bad)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        write(slots[:T], pos=slots[::2], sections=None)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        write(slots[::2], pos=slots[:T], sections=None)
+    assert not kc.float().any() and not vc.float().any()
+    write(slots[:T], w, w)
+    assert kc.float().any() and vc.float().any()
