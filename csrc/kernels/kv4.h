@@ -52,14 +52,15 @@ __device__ __forceinline__ uint32_t fp4x8(const float (&x)[8], float scale) {
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, c[6], c[7], scale, 3);
 }
 
-// A double in 24 bits, the last of them set where the others are not all of it: it is above, below or on every number of
-// fewer bits that the double is above, below or on, so that rounding it on is rounding once.
-__device__ __forceinline__ float round_to_odd(double x) {
-  float f = (float)x;
-  const double back = (double)f;
-  if (back != x) {
+// a + b in 24 bits, the last of them set where the others are not all of it: it is above, below or on every number of
+// fewer bits that the sum is above, below or on, so that rounding it on is rounding once.
+__device__ __forceinline__ float sum_to_odd(double a, double b) {
+  const double s = a + b, t = s - a, rest = (a - (s - t)) + (b - t);   // a + b = s + rest (Knuth's two-sum)
+  float f = (float)s;
+  const double back = (double)f, off = back != s ? s - back : rest;   // what of s is not in f is more than all of rest
+  if (off < 0 || off > 0) {                                            // (neither for infinities and NaN)
     uint32_t u = __float_as_uint(f);
-    if (__builtin_fabs(back) > __builtin_fabs(x)) --u;
+    if ((off < 0) != (u >> 31 != 0)) --u;                              // f is further from zero than the sum
     f = __uint_as_float(u | 1u);
   }
   return f;

@@ -7,9 +7,9 @@
 // for the heads.  A wave has the same heads of 8 tokens (16 with heads of 64), so that its lanes take the same way and a page's
 // rows are written side by side.
 //
-// k is rotated in 64 bits, where the products are exact and the sum is rounded once, and then to the nearest code: a key
-// next to the border of two codes, which are up to a third apart, then has the code that the mathematics gives it, whatever order of
-// operations a compiler prefers.  Values, and keys that are not rotated, are numbers of T already.
+// k is rotated in 64 bits, where the products are exact, and their sum is rounded to odd: the nearest code of that is the nearest code of
+// the exact sum, also where a key lies next to the border of two codes (which are up to a third apart) by less than 64 bits
+// hold, and whatever order of operations a compiler prefers.  Values, and keys that are not rotated, are numbers of T already.
 #include "common.h"
 #include "kv4.h"
 #include "launch.h"
@@ -132,8 +132,8 @@ __global__ __launch_bounds__(KV4_NT) void kv4_write_kernel(
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const double x = xa[j], y = xb[j], co = cc[j], si = sn[j];
-          xa[j] = round_to_odd(__builtin_fma(x, co, -(y * si)));
-          xb[j] = round_to_odd(__builtin_fma(y, co, x * si));
+          xa[j] = sum_to_odd(x * co, -(y * si));
+          xb[j] = sum_to_odd(y * co, x * si);
         }
       }
     }

@@ -95,6 +95,18 @@ def axes_cos_sin(positions: torch.Tensor, cos_sin: torch.Tensor,
     return cos_sin[at, i], cos_sin[at, i + half]
 
 
+def sum_to_odd(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    """a + b in 64 bits, the last one set where the others are not all of it (rounding that on, to
+    fewer bits, is rounding the exact sum)."""
+    s = a + b
+    t = s - a
+    rest = (a - (s - t)) + (b - t)
+    off = (rest < 0) | (rest > 0)
+    u = s.contiguous().view(torch.int64)
+    u = u - (off & ((rest < 0) != (s < 0))).long()
+    return (u | off.long()).view(torch.float64)
+
+
 def rope_qk_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
                      k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor,
                      num_heads: int, num_kv_heads: int, head_dim: int,
@@ -118,11 +130,11 @@ def rope_qk_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.
     if use_rope and (kv4 or sections is not None):
         cos, sin = (c.unsqueeze(1) for c in axes_cos_sin(positions, cos_sin, sections))
 
-        def turn(x, t):
+        def turn(x, t, plus):
             a, b = x.to(t).chunk(2, dim=-1)
-            return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
-        q = turn(q, torch.float32).to(qkv.dtype)
-        k = turn(k, torch.float64) if kv4 else turn(k, torch.float32).to(qkv.dtype)
+            return torch.cat([plus(a * cos, -b * sin), plus(b * cos, a * sin)], dim=-1)
+        q = turn(q, torch.float32, torch.add).to(qkv.dtype)
+        k = turn(k, torch.float64, sum_to_odd) if kv4 else turn(k, torch.float32, torch.add).to(qkv.dtype)
     elif use_rope:
         q = apply_rope(q, positions, cos_sin)
         k = apply_rope(k, positions, cos_sin)

@@ -2,6 +2,7 @@
 several axes, and softmax attention row by row, with how far an implementation may be off.  Written
 apart from the package's own reference."""
 import math
+from fractions import Fraction
 
 import torch
 
@@ -117,3 +118,40 @@ def tables(g, totals, bs, spare=2):
     for i, n in enumerate(need):
         bt[i, :n] = torch.tensor([order.pop() for _ in range(n)], dtype=torch.int32)
     return bt, sum(need) + 1
+
+
+def _nearest_fractions(block):
+    """e2m1 numbers of 32 fractions and their exponent, in rational arithmetic."""
+    most, e = max(abs(x) for x in block), EXPONENTS[torch.float32][0]
+    while most > 7 * Fraction(2) ** e:
+        e += 1
+    out = []
+    for x in block:
+        a = abs(x) / Fraction(2) ** e
+        n = min((0.0, 1.0, 2.0, 4.0, .5, 1.5, 3.0, 6.0), key=lambda n: abs(a - Fraction(n)))   # an even code keeps a tie
+        out.append(math.copysign(n * 2.0 ** e, x))
+    return out, e
+
+
+def keys_beside_borders():
+    """Keys [T, 64] and a row of cos / sin whose rotations lie 2^-60 beside the borders of two codes, on both sides,
+    and beside 7 times the scale: sums of two products that no 64-bit float holds.
+    -> keys, table [1, 64], values [T, 64], exponents [T, 2]."""
+    ties, tiny = [.25, .75, 1.25, 1.75, 2.5, 3.5, 5.0], 2.0 ** -20
+    a = torch.tensor([6.0] + ties * 4 + [0.0] * 3)
+    a[15:29] *= -1
+    b = torch.tensor([0.0] + [-tiny] * 7 + [tiny] * 14 + [-tiny] * 7 + [0.0] * 3)
+    x = torch.stack([a, b]).repeat(4, 1, 1)
+    x[1, :, 0], x[2, :, 0] = torch.tensor([7.0, -tiny]), torch.tensor([7.0, tiny])
+    x[3] = x[3].flip(0)                                       # the small ones first: b + a sin
+    x[3, 0] *= -1
+    table = torch.cat([torch.ones(32), torch.full((32,), 2.0 ** -40)])[None]
+    f = lambda t: [Fraction(v) for v in t.double().tolist()]   # noqa: E731
+    cos, sin = f(table[0, :32]), f(table[0, 32:])
+    v, e = [], []
+    for p, q in ((f(r[0]), f(r[1])) for r in x):
+        one = _nearest_fractions([i * c - j * s for i, j, c, s in zip(p, q, cos, sin)])
+        two = _nearest_fractions([j * c + i * s for i, j, c, s in zip(p, q, cos, sin)])
+        v.append(one[0] + two[0])
+        e.append([one[1], two[1]])
+    return x.view(4, 64), table, torch.tensor(v, dtype=torch.float64), torch.tensor(e, dtype=torch.float64)

@@ -183,3 +183,18 @@ def test_decode_slices_of_a_4bit_cache():
 def test_slices_of_prompts_without_heads():
     """Shapes that the op refuses get there: the host's rule does not divide by their heads."""
     assert ops.kv4_prefill_slices(5, 1, 4, 0, 64, 5000) >= 1 and ops.kv4_prefill_slices(5, 1, 0, 0, 64, 5000) >= 1
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_keys_beside_borders(dt):
+    """The code is the one of the exact sum of the two products, not of its nearest 64-bit number."""
+    x, table, want, e = oracle.keys_beside_borders()
+    assert want[0, 5] == 3.0 and want[0, 12] == 2.0 and e[1, 0] == 1 and e[2, 0] == 0
+    T = len(x)
+    qkv = torch.zeros(T, 3, 64)
+    qkv[:, 1] = x
+    kc, vc = (torch.zeros(ops.kv4_cache_shape(1, 1, 16, 64), dtype=torch.uint8) for _ in range(2))
+    slots = torch.arange(T)
+    ops.rope_kv_write(qkv.to(dt).view(T, -1), slots * 0, table, kc, vc, slots, 1, 1, 64)
+    assert torch.equal(ops.kv4_read(kc, slots, dt)[:, 0].double(), want)
+    assert torch.equal(ref.kv4_parts(kc)[1][0, 0, :T].double() - 127, e)

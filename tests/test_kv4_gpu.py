@@ -673,3 +673,38 @@ def test_axes_refuse_strides_and_norms_of_other_kinds(gpu, cache):
     assert not kc.float().any() and not vc.float().any()
     write(slots[:T], w, w)
     assert kc.float().any() and vc.float().any()
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("T", [4, 40])
+def test_keys_beside_borders(gpu, dt, T):
+    """Keys whose rotation is nearer to a border of two codes than 64 bits hold have the code of the exact sum."""
+    x, table, want, e = oracle.keys_beside_borders()
+    i = torch.arange(T) % len(x)
+    qkv = torch.zeros(T, 3, 64)
+    qkv[:, 1] = x[i]
+    kc, vc = (torch.zeros(ops.kv4_cache_shape(2, 1, 32, 64), dtype=torch.uint8, device=gpu) for _ in range(2))
+    slots = torch.arange(T, device=gpu)
+    ops.rope_kv_write(qkv.to(dt).view(T, -1).to(gpu), slots * 0, table.to(gpu), kc, vc, slots, 1, 1, 64)
+    assert torch.equal(ops.kv4_read(kc, slots, dt)[:, 0].double().cpu(), want[i])
+    scales = ref.kv4_parts(kc.cpu())[1].transpose(1, 2).flatten(0, 1)[:T, 0]
+    assert torch.equal(scales.double() - 127, e[i])
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_rotated_infinities_and_nan(gpu, dt):
+    """Sums beyond 32 bits, of infinities and of NaN are stored as the CPU stores them."""
+    T, d, big = 6, 64, torch.finfo(dt).max
+    x = torch.randn(T, 3, d, generator=_gen(8))
+    x[0, 1, 3], x[1, 1, 35], x[2, 1, 3], x[3, 1, 3], x[3, 1, 35] = float("inf"), -float("inf"), float("nan"), big, big
+    x[4, 1, 3], x[4, 1, 35] = float("inf"), float("inf")
+    x = x.to(dt).view(T, -1)
+    table = torch.cat([torch.full((32,), 2.0 ** 125), torch.full((32,), -2.0 ** 126)])[None]
+    table[0, 8:16], table[0, 40:48] = 2.0 ** -140, 2.0 ** -149           # below 32 bits
+    got = []
+    for dev in (torch.device("cpu"), gpu):
+        kc, vc = (torch.zeros(ops.kv4_cache_shape(1, 1, 16, d), dtype=torch.uint8, device=dev) for _ in range(2))
+        slots = torch.arange(T, device=dev)
+        ops.rope_kv_write(x.to(dev), slots * 0, table.to(dev), kc, vc, slots, 1, 1, d)
+        got.append(ops.kv4_read(kc, slots, dt).cpu())
+    assert torch.equal(*got) and got[0].isfinite().all()
