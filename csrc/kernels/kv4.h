@@ -55,15 +55,16 @@ __device__ __forceinline__ uint32_t fp4x8(const float (&x)[8], float scale) {
 // a + b in 24 bits, the last of them set where the others are not all of it: it is above, below or on every number of
 // fewer bits that the sum is above, below or on, so that rounding it on is rounding once.
 __device__ __forceinline__ float sum_to_odd(double a, double b) {
-  const double s = a + b, t = s - a, rest = (a - (s - t)) + (b - t);   // a + b = s + rest (Knuth's two-sum)
-  float f = (float)s;
-  const double back = (double)f, off = back != s ? s - back : rest;   // what of s is not in f is more than all of rest
-  if (off < 0 || off > 0) {                                            // (neither for infinities and NaN)
-    uint32_t u = __float_as_uint(f);
-    if ((off < 0) != (u >> 31 != 0)) --u;                              // f is further from zero than the sum
-    f = __uint_as_float(u | 1u);
+  const double s = a + b;
+  const uint32_t u = __float_as_uint((float)s);
+  double off = s - (double)__uint_as_float(u);
+  if (off == 0) {                                      // few: what of s is not in 24 bits is more than what of a + b is not in s
+    const double t = s - a;
+    off = (a - (s - t)) + (b - t);                     // a + b = s + off (Knuth's two-sum)
   }
-  return f;
+  // where off's sign is not the sum's, the 24 bits are further from zero than the sum (infinities and NaN: as they are)
+  const uint32_t away = ((uint32_t)(__builtin_bit_cast(uint64_t, off) >> 32) ^ u) >> 31;
+  return __uint_as_float(__builtin_islessgreater(off, 0.0) ? (u - away) | 1u : u);
 }
 
 }  // namespace kgc

@@ -9,7 +9,9 @@
 //
 // k is rotated in 64 bits, where the products are exact, and their sum is rounded to odd: the nearest code of that is the nearest code of
 // the exact sum, also where a key lies next to the border of two codes (which are up to a third apart) by less than 64 bits
-// hold, and whatever order of operations a compiler prefers.  Values, and keys that are not rotated, are numbers of T already.
+// hold, and whatever order of operations a compiler prefers.  (Rounding the sum to 64 bits first takes 95.8 us where this takes 98.5, 16384
+// rows with their reads; one branch for a thread's 16 sums instead of one each keeps more registers: 101.8.)  Values, and keys that are
+// not rotated, are numbers of T already.
 #include "common.h"
 #include "kv4.h"
 #include "launch.h"
