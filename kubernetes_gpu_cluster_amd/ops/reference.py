@@ -95,6 +95,24 @@ def axes_cos_sin(positions: torch.Tensor, cos_sin: torch.Tensor,
     return cos_sin[at, i], cos_sin[at, i + half]
 
 
+def check_sections(positions: torch.Tensor, sections: Sequence[int], cos_sin: torch.Tensor, T: int, d: int,
+                   use_rope: bool) -> None:
+    """What the kernels refuse of positions on several axes."""
+    if not use_rope or not 1 <= len(sections) <= 4:
+        raise ValueError("rope_kv_write: 1 to 4 sections of a rotated head")
+    if positions.shape != (len(sections), T):
+        raise ValueError("rope_kv_write: positions int64 [sections, T]")
+    if cos_sin.shape[0] == 0:
+        raise ValueError("rope_kv_write: an empty cos_sin")
+    if any(not 0 <= n <= d // 2 for n in sections) or sum(sections) != d // 2:
+        raise ValueError(f"rope_kv_write: a section is 0 to d / 2 pairs, all of them {d // 2}, got {list(sections)}")
+
+
+def check_kv4_scales(cache: torch.Tensor, k_scale: float, v_scale: float) -> None:
+    if cache.dtype == torch.uint8 and not k_scale == v_scale == 1.0:
+        raise ValueError("a 4-bit cache has its own scales: k_scale = v_scale = 1")
+
+
 def sum_to_odd(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     """a + b in 64 bits, the last one set where the others are not all of it (rounding that on, to
     fewer bits, is rounding the exact sum)."""
@@ -119,6 +137,9 @@ def rope_qk_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.
     Returns rotated q as a contiguous [T, nq, d] tensor.  A 4-bit cache (uint8) has the codes
     nearest to the exactly rotated k."""
     T = qkv.shape[0]
+    check_kv4_scales(k_cache, k_scale, v_scale)
+    if sections is not None:
+        check_sections(positions, sections, cos_sin, T, head_dim, use_rope)
     qs, ks = num_heads * head_dim, num_kv_heads * head_dim
     q = qkv[:, :qs].reshape(T, num_heads, head_dim)
     k = qkv[:, qs:qs + ks].reshape(T, num_kv_heads, head_dim)
@@ -255,6 +276,7 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
                            block_tables: torch.Tensor, context_lens: torch.Tensor,
                            scale: float, k_scale: float = 1.0, v_scale: float = 1.0) -> torch.Tensor:
     """K1: q [B, nq, d] -> out [B, nq, d], one query token per sequence."""
+    check_kv4_scales(k_cache, k_scale, v_scale)
     B, nq, d = q.shape
     nkv = k_cache.shape[1]
     g = nq // nkv
@@ -277,6 +299,7 @@ def prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     """K2: varlen causal attention for packed prompt chunks.  Sequence i owns query
     rows [qsl[i], qsl[i+1]); its keys are cache positions [0, seq_lens[i]) and its
     queries sit at absolute positions seq_lens[i]-qlen .. seq_lens[i]-1."""
+    check_kv4_scales(k_cache, k_scale, v_scale)
     T, nq, d = q.shape
     nkv = k_cache.shape[1]
     g = nq // nkv

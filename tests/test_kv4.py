@@ -198,3 +198,30 @@ def test_keys_beside_borders(dt):
     ops.rope_kv_write(qkv.to(dt).view(T, -1), slots * 0, table, kc, vc, slots, 1, 1, 64)
     assert torch.equal(ops.kv4_read(kc, slots, dt)[:, 0].double(), want)
     assert torch.equal(ref.kv4_parts(kc)[1][0, 0, :T].double() - 127, e)
+
+
+def test_cpu_forms_refuse_what_the_kernels_refuse():
+    d, T = 64, 3
+    kc, vc = (torch.zeros(ops.kv4_cache_shape(2, 1, 16, d), dtype=torch.uint8) for _ in range(2))
+    table, x, slots = torch.ones(8, d), torch.ones(T, 4 * d, dtype=torch.bfloat16), torch.arange(T)
+    two = torch.zeros(2, T, dtype=torch.int64)
+
+    def no(what, f, *a, **k):
+        with pytest.raises(ValueError, match=what):
+            f(*a, **k)
+
+    def write(pos, table=table, **k):
+        return ops.rope_kv_write(x, pos, table, kc, vc, slots, 2, 1, d, **k)
+    no("own scales", write, slots, k_scale=0.5)
+    no("sections of a rotated head", write, two, sections=(16, 16), use_rope=False)
+    no("1 to 4", write, torch.zeros(5, T, dtype=torch.int64), sections=(28, 1, 1, 1, 1))
+    no("1 to 4", write, torch.zeros(0, T, dtype=torch.int64), sections=())
+    no("all of them 32", write, two, sections=(16, 15))
+    no("0 to d / 2", write, two, sections=(-1, 33))
+    no(r"\[sections, T\]", write, slots, sections=(16, 16))
+    no(r"\[sections, T\]", write, two[:, :2], sections=(16, 16))
+    no("empty cos_sin", write, two, table[:0], sections=(16, 16))
+    assert not kc.any() and not vc.any()
+    q, bt, n = torch.ones(1, 2, d, dtype=torch.bfloat16), torch.zeros(1, 1, dtype=torch.int32), torch.tensor([2])
+    no("own scales", ops.paged_attention_decode, q, kc, vc, bt, n, 1.0, v_scale=2.0)
+    no("own scales", ops.prefill_attention, q, kc, vc, bt, torch.tensor([0, 1]), n, 1.0, k_scale=2.0)
