@@ -155,8 +155,8 @@ void aligned16(const Tensor& t, const char* name) {
 void kv4_write(const Tensor& qkv, int64_t stride, int64_t S, int64_t slice_stride, const Tensor& positions,
                const Tensor& cos_sin, const Tensor& q_out, const Tensor& k_cache, const Tensor& v_cache,
                const Tensor& slot_mapping, const std::optional<Tensor>& q_norm_w, const std::optional<Tensor>& k_norm_w,
-               int64_t T, int64_t nq, int64_t nkv, int64_t d, double eps, bool use_rope, double k_scale, double v_scale,
-               const kgc::RopeAxes& ax) {
+               const std::optional<Tensor>& row_scale, int64_t T, int64_t nq, int64_t nkv, int64_t d, double eps, bool use_rope,
+               double k_scale, double v_scale, const kgc::RopeAxes& ax) {
   check_kv4(k_cache, v_cache, nkv, d, qkv);
   no_kv4_scale(k_scale, v_scale);
   TORCH_CHECK(!use_rope || ax.rows > 0, "kgc.rope_kv_write: an empty cos_sin");
@@ -168,6 +168,13 @@ void kv4_write(const Tensor& qkv, int64_t stride, int64_t S, int64_t slice_strid
   if (q_norm_w.has_value()) {
     w.q_norm_w = q_norm_w->data_ptr();
     w.k_norm_w = k_norm_w->data_ptr();
+  }
+  if (row_scale.has_value()) {
+    TORCH_CHECK(!ax.n, "kgc.rope_kv_write: row_scale without sections");
+    TORCH_CHECK(row_scale->scalar_type() == at::kFloat && row_scale->is_contiguous() && row_scale->numel() == T,
+                "kgc.rope_kv_write: row_scale fp32 [T]");
+    check_same_dev(qkv, *row_scale, "row_scale");
+    w.row_scale = row_scale->data_ptr<float>();
   }
   w.qkv = qkv.data_ptr();
   w.qkv_stride = stride;
@@ -233,7 +240,8 @@ void check_kv4_attention(const Tensor& q, const Tensor& out, const Tensor& k_cac
 void rope_kv_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor q_out, Tensor k_cache,
                    Tensor v_cache, Tensor slot_mapping, std::optional<Tensor> q_norm_w,
                    std::optional<Tensor> k_norm_w, int64_t nq, int64_t nkv, int64_t d,
-                   double eps, bool use_rope, double k_scale, double v_scale, at::OptionalIntArrayRef sections) {
+                   double eps, bool use_rope, double k_scale, double v_scale, at::OptionalIntArrayRef sections,
+                   std::optional<Tensor> row_scale) {
   check_gpu(qkv, "qkv");
   c10::hip::HIPGuardMasqueradingAsCUDA g(qkv.device());
   TORCH_CHECK(d % 16 == 0 && d <= 256, "kgc.rope_kv_write: head_dim");
@@ -279,10 +287,11 @@ void rope_kv_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor q_out, T
               "q_out [T, nq, d] (or empty: k / v only)");
   if (ax.n || kv4) TORCH_CHECK(!kv_only || T == 0 || nq == 0, "kgc.rope_kv_write: 4-bit caches and sections write q too");
   if (kv4) {
-    kv4_write(qkv, stride, S, ss, positions, cos_sin, q_out, k_cache, v_cache, slot_mapping, q_norm_w, k_norm_w, T, nq,
-              nkv, d, eps, use_rope, k_scale, v_scale, ax);
+    kv4_write(qkv, stride, S, ss, positions, cos_sin, q_out, k_cache, v_cache, slot_mapping, q_norm_w, k_norm_w, row_scale,
+              T, nq, nkv, d, eps, use_rope, k_scale, v_scale, ax);
     return;
   }
+  TORCH_CHECK(!row_scale.has_value(), "kgc.rope_kv_write: row_scale is for 4-bit caches");
   TORCH_CHECK(k_cache.is_contiguous() && v_cache.is_contiguous() && k_cache.dim() == 4 &&
               v_cache.dim() == 5 && k_cache.size(1) == nkv && k_cache.size(3) == d &&
               v_cache.size(3) == d && v_cache.size(4) == 8 &&
@@ -3056,7 +3065,7 @@ TORCH_LIBRARY(kgc, m) {
   m.def("rope_kv_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor(a!) q_out, "
         "Tensor(b!) k_cache, Tensor(c!) v_cache, Tensor slot_mapping, Tensor? q_norm_w, "
         "Tensor? k_norm_w, int nq, int nkv, int d, float eps, bool use_rope, float k_scale=1.0, "
-        "float v_scale=1.0, int[]? sections=None) -> ()");
+        "float v_scale=1.0, int[]? sections=None, Tensor? row_scale=None) -> ()");
   m.def("kv4_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor ctx_lens, Tensor(a!)? max_logits, "
         "Tensor(b!)? exp_sums, Tensor(c!)? tmp_out, int Z, float scale) -> Tensor");
   m.def("kv4_prefill(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor query_start_loc, "

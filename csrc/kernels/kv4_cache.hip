@@ -21,12 +21,13 @@ namespace kgc {
 
 constexpr int KV4_NT = 256;
 
-template <typename T, bool NORM, bool ROPE, bool SL, bool AXES, int HG>
+// RS: rows are times row_scale[t] before they are rounded to T (a template: a branch in here costs 2000 rows 20.3 -> 22.1 us).
+template <typename T, bool NORM, bool ROPE, bool SL, bool AXES, int HG, bool RS>
 __global__ __launch_bounds__(KV4_NT) void kv4_write_kernel(
     const void* __restrict__ qkv, int64_t qkv_stride, int S, int64_t slice_stride, const int64_t* __restrict__ positions,
     const float* __restrict__ cos_sin, T* __restrict__ q_out, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
-    const int64_t* __restrict__ slot_mapping, const T* __restrict__ qn_w, const T* __restrict__ kn_w, int64_t T_, int nq,
-    int nkv, int d, int bs, float eps, int num_blocks, RopeAxes ax) {
+    const int64_t* __restrict__ slot_mapping, const T* __restrict__ qn_w, const T* __restrict__ kn_w,
+    const float* __restrict__ row_scale, int64_t T_, int nq, int nkv, int d, int bs, float eps, int num_blocks, RopeAxes ax) {
   const int tph = d >> 4, half = d >> 1;               // threads per head: 4 or 8, whole lane groups
   const int heads = nq + 2 * nkv, groups = (heads + HG - 1) / HG, tpw = 64 / tph;
   const int64_t wave = (int64_t)blockIdx.x * (KV4_NT / 64) + (threadIdx.x >> 6);
@@ -39,15 +40,27 @@ __global__ __launch_bounds__(KV4_NT) void kv4_write_kernel(
   if (slot >= (int64_t)num_blocks * bs) slot = -1;     // beyond the pool: not written
   const int64_t blk = slot >= 0 ? slot / bs : 0;
   const int off = slot >= 0 ? (int)(slot - blk * bs) : 0;
+  float by = 1.f;
+  if constexpr (RS) by = row_scale[t];
   auto load8 = [&](int col) -> u32x4 {
     if constexpr (!SL) {
-      return *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(qkv) + row + col);
+      Pack8<T> o;
+      o.u = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(qkv) + row + col);
+      if constexpr (RS) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o.h[j] = from_f<T>(to_f(o.h[j]) * by);
+      }
+      return o.u;
     } else {
       const float* p = reinterpret_cast<const float*>(qkv) + row + col;
       f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
       for (int z = 1; z < S; ++z) {
         a += *reinterpret_cast<const f32x4*>(p + z * slice_stride);
         b += *reinterpret_cast<const f32x4*>(p + z * slice_stride + 4);
+      }
+      if constexpr (RS) {
+        a *= by;
+        b *= by;
       }
       Pack8<T> o;
 #pragma unroll
@@ -201,13 +214,13 @@ __global__ __launch_bounds__(KV4_NT) void kv4_read_kernel(T* __restrict__ out, c
     if (first + u * KV4_NT < n * per) reinterpret_cast<u32x4*>(out)[first + u * KV4_NT] = fp4x8_widen<T>(w[u], kv4_scale(s[u]));
 }
 
-template <typename T, bool SL, bool AXES, int HG>
+template <typename T, bool SL, bool AXES, int HG, bool RS = false>
 static void kv4_write_norm(const Kv4Write& w, const RopeAxes& ax, int64_t blocks, hipStream_t s) {
 #define KGC_KV4_WRITE(N, R)                                                                                            \
-  kv4_write_kernel<T, N, R, SL, AXES, HG><<<(unsigned)blocks, KV4_NT, 0, s>>>(                                          \
+  kv4_write_kernel<T, N, R, SL, AXES, HG, RS><<<(unsigned)blocks, KV4_NT, 0, s>>>(                                          \
       w.qkv, w.qkv_stride, w.S, w.slice_stride, w.positions, w.cos_sin, (T*)w.q_out, (uint8_t*)w.k_cache,               \
-      (uint8_t*)w.v_cache, w.slots, (const T*)w.q_norm_w, (const T*)w.k_norm_w, w.T, w.nq, w.nkv, w.d, w.bs, w.eps,     \
-      w.num_blocks, ax)
+      (uint8_t*)w.v_cache, w.slots, (const T*)w.q_norm_w, (const T*)w.k_norm_w, w.row_scale, w.T, w.nq, w.nkv, w.d,     \
+      w.bs, w.eps, w.num_blocks, ax)
   if constexpr (AXES) {
     if (w.q_norm_w) KGC_KV4_WRITE(true, true);
     else KGC_KV4_WRITE(false, true);
@@ -225,7 +238,10 @@ template <typename T>
 static void kv4_write_dispatch(const Kv4Write& w, const RopeAxes& ax, hipStream_t s) {
   const int64_t tokens = (w.T * (w.d >> 4) + 63) / 64;           // in waves' worth
   auto blocks = [&](int hg) { return (tokens * ((w.nq + 2 * w.nkv + hg - 1) / hg) + KV4_NT / 64 - 1) / (KV4_NT / 64); };
-  if (w.S > 0) {
+  if (w.row_scale) {                                             // (the host: no sections)
+    if (w.S > 0) kv4_write_norm<T, true, false, 1, true>(w, ax, blocks(1), s);
+    else kv4_write_norm<T, false, false, 1, true>(w, ax, blocks(1), s);
+  } else if (w.S > 0) {
     if (ax.n) kv4_write_norm<T, true, true, 1>(w, ax, blocks(1), s);
     else kv4_write_norm<T, true, false, 1>(w, ax, blocks(1), s);
   } else if (blocks(1) <= 4096) {

@@ -88,6 +88,7 @@ struct Kv4Write {
   void *q_out, *k_cache, *v_cache;
   const int64_t* slots;
   const void *q_norm_w, *k_norm_w;           // nullptr: no q / k RMS norm
+  const float* row_scale;                    // [T]: rows times it before they are rounded to T; nullptr: as they are
   int64_t T;
   int nq, nkv, d, bs, num_blocks;
   float eps;

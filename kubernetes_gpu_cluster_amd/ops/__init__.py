@@ -351,11 +351,10 @@ def paged_attention_decode_rope(qkv: torch.Tensor, positions: torch.Tensor,
                                           k_scale, v_scale)
     sl = qkv.dim() == 3
     if k_cache.dtype == torch.uint8:          # two launches: a 4-bit block's scale is of lanes the decode kernel has elsewhere
-        t = (dtype or qkv.dtype) if sl else qkv.dtype
-        if row_scale is not None:
-            qkv = ((qkv.sum(0) if sl else qkv.float()) * row_scale[:, None]).to(t)
-        q = rope_kv_write(qkv, positions, cos_sin, k_cache, v_cache, slot_mapping, num_heads, num_kv_heads,
-                          head_dim, q_norm_w, k_norm_w, eps, use_rope, k_scale, v_scale, t)
+        q = qkv.new_empty((qkv.shape[1] if sl else qkv.shape[0], num_heads, head_dim),
+                          dtype=(dtype or qkv.dtype) if sl else qkv.dtype)
+        _k().rope_kv_write(qkv, positions, cos_sin, q, k_cache, v_cache, slot_mapping, q_norm_w, k_norm_w, num_heads,
+                           num_kv_heads, head_dim, eps, use_rope, k_scale, v_scale, None, row_scale)
         return paged_attention_decode(q, k_cache, v_cache, block_tables, context_lens, scale, workspace, grid_z,
                                       k_scale=k_scale, v_scale=v_scale)
     B = qkv.shape[1] if sl else qkv.shape[0]

@@ -708,3 +708,59 @@ def test_rotated_infinities_and_nan(gpu, dt):
         ops.rope_kv_write(x.to(dev), slots * 0, table.to(dev), kc, vc, slots, 1, 1, d)
         got.append(ops.kv4_read(kc, slots, dt).cpu())
     assert torch.equal(*got) and got[0].isfinite().all()
+
+
+def _launched(f):
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        f()
+        torch.cuda.synchronize()
+    return [e.key for e in prof.key_averages() if e.device_type == torch.autograd.DeviceType.CUDA]
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("S,norms", [(0, False), (3, False), (8, True), (0, True)])
+def test_decode_step_with_row_scales(gpu, dt, S, norms):
+    """A decode step's projection times a number per row before its rounding, in the launch that rotates: as the same step
+    over the rows that fp32 sums, the product and one rounding give, and in two launches."""
+    g, B, nq, nkv, d, bs = _gen(S + 17), 9, 8, 2, 128, 32
+    x = torch.randn(max(S, 1), B, (nq + 2 * nkv) * d, generator=g)
+    x = x if S else x[0].to(dt)
+    r = torch.rand(B, generator=g) + 0.5
+    rows = x.float() if not S else x[0]
+    for z in range(1, S):
+        rows = rows + x[z]
+    rows = (rows * r[:, None]).to(dt)
+    ctx = [1 + 29 * i for i in range(B)]
+    bt, nb = oracle.tables(g, ctx, bs)
+    kc, vc = (oracle.random_cache(g, nb, nkv, bs, d, dt) for _ in range(2))
+    slots = torch.tensor([int(bt[i, (n - 1) // bs]) * bs + (n - 1) % bs for i, n in enumerate(ctx)])
+    w = [torch.rand(d, generator=g).add(0.5).to(dt).to(gpu) for _ in range(2)] if norms else [None, None]
+    pos, table = torch.tensor(ctx, device=gpu) - 1, ref.rope_cos_sin_cache(d, 300, 10000.0).to(gpu)
+
+    def step(qkv, caches, **k):
+        return ops.paged_attention_decode_rope(qkv, pos, table, *caches, slots.to(gpu), nq, nkv, d, bt.to(gpu),
+                                               (pos + 1).int(), d ** -0.5, *w, dtype=dt, **k)
+    got, want = ([c.to(gpu) for c in (kc, vc)] for _ in range(2))
+    a, b = step(x.to(gpu), got, row_scale=r.to(gpu)), step(rows.to(gpu), want)
+    assert torch.equal(a, b) and all(torch.equal(p, q) for p, q in zip(got, want))
+    xg, rg = x.to(gpu), r.to(gpu)
+    names = _launched(lambda: step(xg, got, row_scale=rg))
+    assert sum("kv4_" in n for n in names) == 2 and not any("reduce" in n for n in names), names
+
+
+def test_row_scales_refused(gpu):
+    d, T, bf = 128, 3, torch.bfloat16
+    kc, vc = (torch.zeros(ops.kv4_cache_shape(2, 1, 16, d), dtype=torch.uint8, device=gpu) for _ in range(2))
+    x, table = torch.zeros(T, 4 * d, dtype=bf, device=gpu), torch.zeros(8, d, device=gpu)
+    pos, n = torch.arange(T, device=gpu), torch.ones(T, dtype=torch.int32, device=gpu)
+    bt, r = torch.zeros(T, 1, dtype=torch.int32, device=gpu), torch.ones(2 * T, device=gpu)
+    for bad in (r, r[::2], r[:T].double(), r[:T].cpu()):
+        with pytest.raises(RuntimeError, match="row_scale"):
+            ops.paged_attention_decode_rope(x, pos, table, kc, vc, pos, 2, 1, d, bt, n, 1.0, row_scale=bad)
+    wide = torch.zeros(2, 1, 16, d, dtype=bf, device=gpu), torch.zeros(2, 1, 2, d, 8, dtype=bf, device=gpu)
+    with pytest.raises(RuntimeError, match="4-bit caches"):
+        torch.ops.kgc.rope_kv_write(x, pos, table, torch.empty(T, 2, d, dtype=bf, device=gpu), *wide, pos, None, None, 2, 1, d,
+                                    1e-6, True, 1.0, 1.0, None, r[:T])
+    with pytest.raises(RuntimeError, match="without sections"):
+        torch.ops.kgc.rope_kv_write(x, pos[None], table, torch.empty(T, 2, d, dtype=bf, device=gpu), kc, vc, pos, None, None, 2, 1,
+                                    d, 1e-6, True, 1.0, 1.0, [64], r[:T])
