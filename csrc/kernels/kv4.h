@@ -67,4 +67,12 @@ __device__ __forceinline__ float sum_to_odd(double a, double b) {
   return __uint_as_float(__builtin_islessgreater(off, 0.0) ? (u - away) | 1u : u);
 }
 
+// l + the two numbers of T in w
+template <typename T> __device__ __forceinline__ float kv4_add_pair(uint32_t w, float l) {
+  if constexpr (std::is_same_v<T, bf16>)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), bf16x2_t{(bf16)1.f, (bf16)1.f}, l, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), f16x2_t{(f16)1.f, (f16)1.f}, l, false);
+}
+
 }  // namespace kgc

@@ -154,16 +154,15 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_decode_kernel(
     }
     // a row none of whose scores is above -inf (q or k too large): no difference of infinities
     const float ref = m_run == -INFINITY ? 0.f : m_run;
-    // probabilities are rounded to T for the product, as the keys' and values' type has it; their sum is not
+    // probabilities are rounded to T for the product, as the keys' and values' type has it; the sum, in 32 bits, is that of the
+    // rounded ones, so that they add up to one
     Pack8<T> pf;
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = __builtin_amdgcn_exp2f(sc[g][i] - ref);
-        l_run += p;
-        pf.h[4 * g + i] = from_f<T>(p);
-      }
+      for (int i = 0; i < 4; ++i) pf.h[4 * g + i] = from_f<T>(__builtin_amdgcn_exp2f(sc[g][i] - ref));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l_run = kv4_add_pair<T>(pf.u[i], l_run);
 #pragma unroll
     for (int t = 0; t < DT; ++t) {
       const T* src = lds_v + (4 * qd + (r16 >> 2)) * VS + 16 * t + 4 * (r16 & 3);

@@ -30,14 +30,6 @@ __device__ __forceinline__ float kv4_max_pair(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// l + the two numbers of T in w
-template <typename T> __device__ __forceinline__ float kv4_add_pair(uint32_t w, float l) {
-  if constexpr (std::is_same_v<T, bf16>)
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), bf16x2_t{(bf16)1.f, (bf16)1.f}, l, false);
-  else
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), f16x2_t{(f16)1.f, (f16)1.f}, l, false);
-}
-
 template <typename T, int D, int GH, int BUFS>
 __global__ __launch_bounds__(256, BUFS == 2 ? 2 : D == 128 ? 3 : 4) void kv4_prefill_kernel(
     const T* __restrict__ q, T* __restrict__ out, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,

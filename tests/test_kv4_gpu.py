@@ -1,4 +1,6 @@
 """The 4-bit cache's kernels (csrc/kernels/kv4_*.hip) and rotary positions on several axes against 64 bits."""
+import math
+
 import pytest
 import torch
 
@@ -764,3 +766,25 @@ def test_row_scales_refused(gpu):
     with pytest.raises(RuntimeError, match="without sections"):
         torch.ops.kgc.rope_kv_write(x, pos[None], table, torch.empty(T, 2, d, dtype=bf, device=gpu), kc, vc, pos, None, None, 2, 1,
                                     d, 1e-6, True, 1.0, 1.0, [64], r[:T])
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("B,z", [(3, 1), (3, 3), (70, 1)])
+def test_values_that_are_alike_come_back(gpu, dt, B, z):
+    """Weights add up to one as they are rounded: with values that are all 1 the result is 1, whatever the weights' rounding.
+    Of every 32 keys 31 have a weight just below the middle between a half and the type's next number.  (Numerator and
+    denominator are sums of the same 400 or fewer numbers: 2^-15 apart at most, an eighth of half of fp16's step.)"""
+    n, d, u = 400, 64, torch.finfo(dt).eps / 2
+    kc, vc = (torch.zeros(ops.kv4_cache_shape(14, 1, 32, d), dtype=torch.uint8, device=gpu) for _ in range(2))
+    for c in (kc, vc):
+        ref.kv4_parts(c)[1].fill_(127)
+    ref.kv4_parts(vc)[0].fill_(0x22)
+    ref.kv4_parts(kc)[0][:, :, 1:, 0] = 0xA                   # -1 in the first element
+    q = torch.zeros(B, 2, d, dtype=dt, device=gpu)
+    q[..., 0] = 1
+    scale = math.log(2) - math.log1p(0.98 * u)
+    bt = torch.arange(14, dtype=torch.int32, device=gpu).expand(B, 14).contiguous()
+    ctx = torch.tensor([n, 200, 333] + [n - i for i in range(B - 3)], dtype=torch.int32, device=gpu)
+    assert (ops.paged_attention_decode(q, kc, vc, bt, ctx, scale, None, z) == 1).all()
+    starts = torch.arange(B + 1, dtype=torch.int32, device=gpu)
+    assert (ops.prefill_attention(q, kc, vc, bt, starts, ctx, scale) == 1).all()
