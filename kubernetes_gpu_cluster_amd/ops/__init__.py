@@ -312,7 +312,7 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         if k_cache.dtype == torch.uint8 and k_scale == v_scale == 1.0:       # one call, allocations and all
             ml, es, tmp = workspace or (None, None, None)
             return _k().kv4_decode(q, k_cache, v_cache, block_tables, context_lens, ml, es, tmp,
-                                   min(grid_z, _decode_z_cap(workspace, B, nq)) if workspace else grid_z, scale)
+                                   min(grid_z, _decode_z_cap(workspace, B, nq) if workspace else 1024), scale)
         out = torch.empty_like(q)
     if workspace is None:
         workspace = decode_partials(B, nq, d, block_tables.shape[1], k_cache.shape[2], q.device)

@@ -788,3 +788,15 @@ def test_values_that_are_alike_come_back(gpu, dt, B, z):
     assert (ops.paged_attention_decode(q, kc, vc, bt, ctx, scale, None, z) == 1).all()
     starts = torch.arange(B + 1, dtype=torch.int32, device=gpu)
     assert (ops.prefill_attention(q, kc, vc, bt, starts, ctx, scale) == 1).all()
+
+
+@pytest.mark.parametrize("z", [1024, 1025, 5000])
+def test_decode_of_more_slices_than_a_merge_takes(gpu, z):
+    """Slices beyond the merge's 1024 are 1024, as over the wider caches; 0 are refused."""
+    ctx = [700, 1, 300]
+    q, kc, vc, bt, _ = _attention_case(4, 4, 2, 64, 32, torch.bfloat16, [1] * 3, [c - 1 for c in ctx])
+    a = [t.to(gpu) for t in (q, kc, vc, bt, torch.tensor(ctx, dtype=torch.int32))]
+    got = ops.paged_attention_decode(*a, 0.125, None, z)
+    _check_attention(got.cpu(), q, kc, vc, bt, [1] * 3, ctx, 0.125)
+    with pytest.raises(RuntimeError, match="Z"):
+        ops.paged_attention_decode(*a, 0.125, None, 0)
