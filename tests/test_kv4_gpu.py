@@ -800,3 +800,63 @@ def test_decode_of_more_slices_than_a_merge_takes(gpu, z):
     _check_attention(got.cpu(), q, kc, vc, bt, [1] * 3, ctx, 0.125)
     with pytest.raises(RuntimeError, match="Z"):
         ops.paged_attention_decode(*a, 0.125, None, 0)
+
+
+# ------------------------------------------------------------------ the forms that large steps take
+def _ran(names, kernel, *args):
+    """Whether a kernel's form with these last template arguments is among the launched ones; the profiler has names mangled or
+    plain (the 16-bit types are beyond some demanglers)."""
+    raw = "".join(f"Lb{int(a)}E" if isinstance(a, bool) else f"Li{a}E" for a in args) + "EEv"
+    plain = ", ".join(str(a).lower() for a in args) + ">"
+    return any(kernel in n and (raw in n or plain in n) for n in names)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("nq,nkv,d,bs,T,sections", [
+    (32, 8, 128, 32, 2800, None),
+    (32, 8, 128, 32, 2733, (10, 9, -1)),
+    (15, 5, 128, 16, 5300, None),                              # 25 heads: the last four are one
+    (15, 5, 128, 64, 5250, (5, -1)),
+    (12, 12, 64, 32, 7300, None),
+    (13, 5, 64, 32, 11500, (-1,)),                             # 23 heads: the last four are three
+])
+def test_write_of_many_rows(gpu, dt, nq, nkv, d, bs, T, sections):
+    """More than 4096 workgroups of a head per thread: four heads per thread (kv4_cache.hip kv4_write_dispatch)."""
+    names = _launched(lambda: test_write(gpu, dt, nq, nkv, d, bs, T, sections, 0))
+    assert _ran(names, "kv4_write_kernel", True, False, sections is not None, 4, False), names
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("rope,norms", [(True, True), (False, True), (False, False)])
+def test_write_of_many_rows_normed_and_unrotated(gpu, dt, rope, norms):
+    """Four heads per thread write what a head per thread writes: the same rows in one call and in calls of 500."""
+    g, nq, nkv, d, bs, T = _gen(3), 30, 7, 128, 32, 3500
+    x = torch.randn(T, (nq + 2 * nkv) * d, generator=g).to(dt).to(gpu)
+    w = [torch.rand(d, generator=g).add(0.5).to(dt).to(gpu) for _ in range(2)] if norms else [None, None]
+    pos, table = torch.randint(0, 300, (T,), generator=g).to(gpu), ref.rope_cos_sin_cache(d, 300, 10000.0).to(gpu)
+    slots = torch.randperm(T + 60, generator=g)[:T].to(gpu)
+    slots[5] = -1
+    got = []
+
+    def write(step):
+        caches = [torch.zeros(ops.kv4_cache_shape(-(-(T + 60) // bs), nkv, bs, d), dtype=torch.uint8, device=gpu) for _ in range(2)]
+        q = [ops.rope_kv_write(x[a:a + step], pos[a:a + step], table, *caches, slots[a:a + step], nq, nkv, d, *w, use_rope=rope)
+             for a in range(0, T, step)]
+        got.append([torch.cat(q), *caches])
+    for step, heads in ((T, 4), (500, 1)):
+        names = _launched(lambda: write(step))
+        assert _ran(names, "kv4_write_kernel", rope, False, False, heads, False), names
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and got[0][1].any()
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("nkv,d,n", [(8, 128, 8200), (12, 64, 10950), (1, 128, 65601), (8, 128, 8190)])
+def test_read_of_many_rows(gpu, dt, nkv, d, n):
+    """2^20 pieces of 8 elements and more are read four per thread (the last case: just fewer)."""
+    g = _gen(n)
+    c = oracle.random_cache(g, 70, nkv, 16, d, dt)
+    slots = torch.randint(0, 70 * 16, (n,), generator=g)
+    slots[3], slots[n // 2], slots[n - 1] = -1, 70 * 16, 1 << 40
+    assert (n * nkv * (d // 8) >= 1 << 20) == (n != 8190)
+    got = ops.kv4_read(c.to(gpu), slots.to(gpu), dt).cpu()
+    assert torch.equal(got, ref.kv4_read(c, slots, dt))
