@@ -860,3 +860,55 @@ def test_read_of_many_rows(gpu, dt, nkv, d, n):
     assert (n * nkv * (d // 8) >= 1 << 20) == (n != 8190)
     got = ops.kv4_read(c.to(gpu), slots.to(gpu), dt).cpu()
     assert torch.equal(got, ref.kv4_read(c, slots, dt))
+
+
+def _attention_wanted(q, kc, vc, bt, new, totals, scale):
+    """What _check_attention compares with, once for several calls: results and how far off, [rows, heads, d]."""
+    nq, nkv = q.shape[1], kc.shape[1]
+    want, tol, at = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64), 0
+    for i, (m, n) in enumerate(zip(new, totals)):
+        seen = torch.arange(n)[None] <= torch.arange(n - m, n)[:, None]
+        for h in range(nkv if n else 0):
+            k, v = (oracle.rows(c, bt[i], n, h, q.shape[2]) for c in (kc, vc))
+            g = nq // nkv                                     # a group's rows at once
+            rows = q[at:at + m, h * g:(h + 1) * g].transpose(0, 1).flatten(0, 1)
+            o, t = oracle.attend(rows, k, v, scale, seen.repeat(g, 1), q.dtype)
+            for to, x in ((want, o), (tol, t)):
+                to[at:at + m, h * g:(h + 1) * g] = x.view(g, m, -1).transpose(0, 1)
+        at += m
+    return want, tol
+
+
+# The waves of a workgroup go by the (sequence, kv head) pairs: fewer than 64 four, to 511 eight, to 1023 four, to 1535 two, then one
+DECODE_FORMS = [
+    # waves, q heads, kv heads, head, page, contexts
+    (8, 32, 8, 128, 32, [700, 1, 0, 33, 320, 64, 511, 2300, 90]),
+    (8, 16, 1, 128, 16, [1 + 37 * i % 500 for i in range(66)]),
+    (8, 6, 2, 128, 64, [700 - 19 * i for i in range(36)]),
+    (8, 10, 2, 64, 32, [2 + 41 * i % 800 for i in range(40)] + [2500]),
+    (4, 32, 8, 128, 32, [1 + 53 * i % 900 for i in range(70)] + [2100]),
+    (4, 15, 5, 64, 16, [600 - 5 * i for i in range(105)]),
+    (2, 32, 8, 128, 32, [61 * i % 700 for i in range(129)] + [2300]),
+    (2, 12, 4, 64, 32, [1 + 43 * i % 500 for i in range(260)]),
+    (1, 32, 8, 128, 32, [59 * i % 650 for i in range(199)] + [2200]),
+    (1, 12, 2, 128, 16, [1 + 31 * i % 300 for i in range(770)]),
+    (1, 8, 4, 64, 64, [47 * i % 400 for i in range(399)] + [2400]),
+]
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("waves,nq,nkv,d,bs,ctx", DECODE_FORMS)
+def test_decode_by_waves(gpu, dt, waves, nq, nkv, d, bs, ctx):
+    """Every number of waves, over contexts that take several turns of their loops, with heads that share a kv head, whole and
+    in slices."""
+    B = len(ctx)
+    q, kc, vc, bt, _ = _attention_case(B + d, nq, nkv, d, bs, dt, [1] * B, [c - 1 for c in ctx])
+    want, tol = _attention_wanted(q, kc, vc, bt, [1] * B, ctx, d ** -0.5)
+    a = [t.to(gpu) for t in (q, kc, vc, bt, torch.tensor(ctx, dtype=torch.int32))]
+    rule = ops.decode_grid_z(B, nkv, max(ctx), cache_dtype=torch.uint8)
+    assert ops.kv4_decode_waves(B * nkv) == waves
+    for z in sorted({1, 2, 5, rule}):
+        got = []
+        names = _launched(lambda: got.append(ops.paged_attention_decode(*a, d ** -0.5, None, z)))
+        assert _ran(names, "kv4_decode_kernel", d, waves) and any("paged_decode_reduce" in n for n in names) == (z > 1), names
+        assert ((got[0].cpu().double() - want).abs() <= tol).all(), z
