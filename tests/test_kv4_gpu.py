@@ -912,3 +912,34 @@ def test_decode_by_waves(gpu, dt, waves, nq, nkv, d, bs, ctx):
         names = _launched(lambda: got.append(ops.paged_attention_decode(*a, d ** -0.5, None, z)))
         assert _ran(names, "kv4_decode_kernel", d, waves) and any("paged_decode_reduce" in n for n in names) == (z > 1), names
         assert ((got[0].cpu().double() - want).abs() <= tol).all(), z
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("nq,nkv,d,bs,new,old,heads", [
+    (32, 8, 128, 32, [300, 33, 1], [2000, 700, 0], 4),
+    (12, 12, 64, 16, [301, 280, 226], [1500, 1400, 20], 1),
+    (12, 6, 128, 64, [290, 129, 140], [0, 1900, 450], 2),
+    (24, 2, 64, 32, [200, 127, 1, 260], [1100, 90, 800, 0], 4),
+])
+@pytest.mark.parametrize("z", [8, 13, 32])
+def test_prompts_in_slices_by_many_workgroups(gpu, dt, nq, nkv, d, bs, new, old, heads, z):
+    """Slices that come to more than two workgroups per CU (512 here): one LDS buffer per tile."""
+    if torch.cuda.get_device_properties(gpu).multi_processor_count != 256:
+        pytest.skip("lines for 256 CUs")
+    assert sum(-(-n // 128) for n in new) * nq * z > 512
+    names = _launched(lambda: test_prompts_in_slices(gpu, dt, nq, nkv, d, bs, new, old, z))
+    assert _ran(names, "kv4_prefill_kernel", heads, 1) and any("kv4_prefill_merge" in n for n in names), names
+
+
+def test_slices_that_the_rule_gives(gpu):
+    """The public call's own slices where they come to many workgroups, with a result of its own and one of the caller's."""
+    new, old, nq, nkv, d = [301, 264, 227], [7000, 6500, 3000], 12, 12, 64
+    q, kc, vc, bt, totals = _attention_case(5, nq, nkv, d, 32, torch.float16, new, old)
+    assert ops.kv4_prefill_slices(sum(new), 3, nq, nkv, d, max(totals)) > 1
+    want, tol = _attention_wanted(q, kc, vc, bt, new, totals, d ** -0.5)
+    a = [t.to(gpu) for t in (q, kc, vc, bt, _starts(new), torch.tensor(totals, dtype=torch.int32))]
+    for out in (None, torch.full_like(a[0], 7)):
+        got = []
+        names = _launched(lambda: got.append(ops.prefill_attention(*a, d ** -0.5, out=out)))
+        assert any("kv4_prefill_merge" in n for n in names) and (out is None or got[0] is out)
+        assert ((got[0].cpu().double() - want).abs() <= tol).all()
