@@ -943,3 +943,40 @@ def test_slices_that_the_rule_gives(gpu):
         names = _launched(lambda: got.append(ops.prefill_attention(*a, d ** -0.5, out=out)))
         assert any("kv4_prefill_merge" in n for n in names) and (out is None or got[0] is out)
         assert ((got[0].cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("cache", ["auto", "fp8"])
+@pytest.mark.parametrize("nq,nkv,d,bs,T,sections,by_rows", [
+    (12, 12, 64, 32, 1400, (8, 12, 12), True),
+    (12, 12, 64, 32, 1300, (8, 12, 12), False),               # fewer than 3M elements: a launch
+    (25, 5, 64, 16, 2001, (3, 0, 20, 9), True),               # 30 heads of q and k: the last four are two
+    (5, 1, 64, 24, 7100, (32,), True),
+    (33, 3, 128, 16, 700, (50, 14), True),
+])
+def test_axes_of_many_rows(gpu, dt, cache, nq, nkv, d, bs, T, sections, by_rows):
+    """q and k by rows and v by 8-row groups, from 3 * 2^20 elements on, as the one-position kernel turns each axis's pairs."""
+    g, t = _gen(T), torch.float8_e4m3fn if cache == "fp8" else dt
+    nb = T // bs + 3
+    mk = lambda: (torch.zeros(nb, nkv, bs, d).to(t).to(gpu), torch.zeros(nb, nkv, bs // 8, d, 8).to(t).to(gpu))   # noqa: E731
+    x = torch.randn(T, (nq + 2 * nkv) * d, generator=g).to(dt).to(gpu)
+    table = ref.rope_cos_sin_cache(d, 90, 10000.0)
+    pos = torch.randint(-5, 99, (len(sections), T), generator=g)
+    slots = torch.arange(T) + 5                               # runs that start in an 8-key group, one that ends in one, and padding
+    slots[100:] += 3
+    slots[-3:] = -1
+    slots = slots.to(gpu)
+    kc, vc = mk()
+    q = []
+    names = _launched(lambda: q.append(ops.rope_kv_write(x, pos.to(gpu), table.to(gpu), kc, vc, slots, nq, nkv, d,
+                                                         sections=sections)))
+    assert any("rope_rows_kernel" in n for n in names) == any("kv_group_kernel" in n for n in names) == by_rows, names
+    for a, n in enumerate(sections):
+        rows = table[pos[a].clamp(0, 89)].contiguous().to(gpu)
+        k2, v2 = mk()
+        q2 = ops.rope_kv_write(x, torch.arange(T, device=gpu), rows, k2, v2, slots, nq, nkv, d)
+        i = torch.arange(sum(sections[:a]), sum(sections[:a + 1]), device=gpu)
+        i = torch.cat([i, i + d // 2])
+        assert torch.equal(q[0][..., i], q2[..., i])
+        assert torch.equal(kc.float()[..., i], k2.float()[..., i]) and torch.equal(vc.float(), v2.float())
+    assert vc.float().any() and kc.float().any()
