@@ -980,3 +980,30 @@ def test_axes_of_many_rows(gpu, dt, cache, nq, nkv, d, bs, T, sections, by_rows)
         assert torch.equal(q[0][..., i], q2[..., i])
         assert torch.equal(kc.float()[..., i], k2.float()[..., i]) and torch.equal(vc.float(), v2.float())
     assert vc.float().any() and kc.float().any()
+
+
+@pytest.mark.parametrize("eager", [False, True])
+def test_engine_of_learned_positions(gpu, eager):
+    """OPT over a 4-bit cache: heads of 64, one q head per kv head, nothing rotated.  Prompts in chunks and decode steps run, and
+    every layer's pages hold what was written."""
+    from kubernetes_gpu_cluster_amd.engine.llm_engine import LLM
+    from kubernetes_gpu_cluster_amd.engine.sequence import SamplingParams
+    from kubernetes_gpu_cluster_amd.models import configs
+    configs.PRESETS["opt-125m-two"] = configs.PRESETS["opt-125m"].shrink(name="opt-125m-two", num_layers=2)
+    try:
+        llm = LLM("opt-125m-two", device="cuda", dtype="float16", random_init=True, seed=2, max_model_len=256, max_num_seqs=4,
+                  max_num_batched_tokens=64, num_gpu_blocks_override=64, kv_cache_dtype="fp4", enforce_eager=eager)
+    finally:
+        del configs.PRESETS["opt-125m-two"]
+    r = llm.engine.executor.runner
+    assert r.kv.dtype == torch.uint8 and r.kv.shape[:2] == (2, 2)
+    outs = llm.generate([[5 + i, 6, 7, 8, 9] * 9 for i in range(3)],
+                        SamplingParams(temperature=0, max_tokens=6, ignore_eos=True, logprobs=5))
+    assert (r.stats["graph_steps"] > 0) == (not eager)
+    for o in outs:
+        assert len(o.output_token_ids) == 6 and all(math.isfinite(p) for step in o.logprobs for _, p in step[2])
+    # 3 prompts of 45 tokens and five of their answers' six: rows with a scale of their own
+    for layer in r.kv:
+        for c in layer:
+            assert int((ref.kv4_parts(c)[1] != 0).all(-1).all(1).sum()) == 3 * 50
+    llm.shutdown()
