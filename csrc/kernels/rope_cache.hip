@@ -86,6 +86,7 @@ __global__ __launch_bounds__(ROPE_NT) void rope_kv_kernel(
   const int it = blockIdx.y * ROPE_NT + threadIdx.x;
   int64_t slot = slot_mapping[t];
   KGC_DCHECK_RANGE(slot, -1, (int64_t)num_blocks * bs, "KV slot");   // -1: no KV write
+  if (AXES && slot >= (int64_t)num_blocks * bs) slot = -1;
   const int64_t row = (int64_t)t * qkv_stride;   // element offset of this token's row
   const int64_t blk = slot >= 0 ? slot / bs : 0;
   const int off = slot >= 0 ? (int)(slot % bs) : 0;
@@ -246,7 +247,7 @@ __global__ __launch_bounds__(KVG_NT) void kv_group_kernel(
   if (lane < 22 && row >= 0 && row < T_) {
     int64_t sl = slot_mapping[row];
     KGC_DCHECK_RANGE(sl, -1, (int64_t)num_blocks * bs, "KV slot");
-    slot = sl < 0 ? -1 : (int)sl;
+    slot = sl < 0 || (VONLY && sl >= (int64_t)num_blocks * bs) ? -1 : (int)sl;
     if (!VONLY && slot >= 0) pos = (int)positions[row];
   }
   const int up = __shfl_down(slot, 1, 64);
@@ -386,6 +387,7 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(
   }
   int64_t slot = slot_mapping[t];
   KGC_DCHECK_RANGE(slot, -1, (int64_t)num_blocks * bs, "KV slot");
+  if (slot >= (int64_t)num_blocks * bs) slot = -1;
   float cc[8], sn[8];
   axes_cos_sin(ax, positions, (int)t, cos_sin, d, c * 8, cc, sn);
 #pragma unroll

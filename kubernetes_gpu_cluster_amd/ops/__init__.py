@@ -147,6 +147,7 @@ def rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Ten
     Slots are distinct (-1: no write).  ``sections``: positions are int64 [A, T], one row per axis (time, height, width),
     and pair i of a head turns by the axis whose section holds i -- pairs per axis, one after the
     other, head_dim / 2 in all, 4 axes at most; positions outside ``cos_sin`` take its nearest row.
+    Over 4-bit caches and with sections a slot beyond the pool is not written.
     On the GPU ``qkv`` may also be the K9m split-K slices of the QKV
     projection (fp32 [S, T, N], ops/gemm.py linear_qkv): the kernel sums them, and
     ``dtype`` names the activation dtype of q."""

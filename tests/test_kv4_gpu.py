@@ -1007,3 +1007,28 @@ def test_engine_of_learned_positions(gpu, eager):
         for c in layer:
             assert int((ref.kv4_parts(c)[1] != 0).all(-1).all(1).sum()) == 3 * 50
     llm.shutdown()
+
+
+@pytest.mark.parametrize("cache", ["auto", "fp8"])
+@pytest.mark.parametrize("T,slices", [(40, 0), (40, 2), (1400, 0)])
+def test_axes_leave_out_slots_beyond_the_pool(gpu, cache, T, slices):
+    """As the 4-bit write does, in one launch and by rows and 8-row groups; pages behind the pool in the same allocation stay."""
+    if ops.DEBUG:
+        pytest.skip("the bounds-checking build reports them")
+    g, dt, nq, nkv, d, bs = _gen(6), torch.bfloat16, 12, 12, 64, 32
+    t, nb = torch.float8_e4m3fn if cache == "fp8" else dt, T // bs + 2
+    x = torch.randn(max(slices, 1), T, (nq + 2 * nkv) * d, generator=g)
+    x = x.to(gpu) if slices else x[0].to(dt).to(gpu)
+    table = ref.rope_cos_sin_cache(d, 90, 10000.0).to(gpu)
+    pos = torch.randint(0, 90, (2, T), generator=g).to(gpu)
+    good = torch.arange(T) + 3
+    bad = good.clone()
+    for i, s in ((5, nb * bs), (9, nb * bs + 17), (17, 1 << 40), (T - 1, -7), (T - 2, 2 ** 31 + 5)):
+        bad[i], good[i] = s, -1
+    got = []
+    for slots in (good, bad):
+        k_all, v_all = torch.zeros(nb + 3, nkv, bs, d, device=gpu).to(t), torch.zeros(nb + 3, nkv, bs // 8, d, 8, device=gpu).to(t)
+        q = ops.rope_kv_write(x, pos, table, k_all[:nb], v_all[:nb], slots.to(gpu), nq, nkv, d, dtype=dt, sections=(12, 20))
+        got.append([q, k_all.float(), v_all.float()])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert got[0][1].any() and not got[1][1][nb:].any() and not got[1][2][nb:].any()
