@@ -246,8 +246,8 @@ static void kv4_write_dispatch(const Kv4Write& w, const RopeAxes& ax, hipStream_
     else kv4_write_norm<T, true, false, 1>(w, ax, blocks(1), s);
   } else if (blocks(1) <= 4096) {
     // Few workgroups: a head per thread, all loads of a call on their way at once; many: cos / sin for four.  us with both
-    // caches' rows read back, one head -> four: 256 rows of 32 / 8 heads 9.4 -> 12.1, 1000 12.8 -> 15.0, 2000 20.0 -> 19.6, 16384
-    // 100.5 -> 97.6 (the write alone 75, 353 MB); 4000 of 12 / 12 heads of 64 18.0 -> 21.0.
+    // caches' rows read back, one head -> four: 256 rows of 32 / 8 heads 9.2 -> 12.7, 1000 13.4 -> 16.2, 2000 20.2 -> 20.2, 2700 26.3
+    // -> 25.9, 4000 33.9 -> 34.2, 16384 107 -> 98.0 (the write alone 77, 353 MB); 4000 of 12 / 12 heads of 64 19.7 -> 23.3.
     if (ax.n) kv4_write_norm<T, false, true, 1>(w, ax, blocks(1), s);
     else kv4_write_norm<T, false, false, 1>(w, ax, blocks(1), s);
   } else if (ax.n) {

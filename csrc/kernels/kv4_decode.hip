@@ -2,8 +2,9 @@
 //
 // A workgroup of NW waves per (sequence, kv head, z-slice), with the slices and the merge of paged_decode_wave_kernel
 // (decode_slices.h, attention_decode.hip); its waves share the slice's chunks and merge in LDS, so that most calls are one
-// launch.  A chunk is 32 tokens, two groups of 16; a page holds 16 or more, so that a group lies in one.  Lane (token r16 of a group, quarter qd of the head) loads its quarter row with one load of D / 8 bytes, and the
-// scale with it; next chunk's loads are on their way while one computes.
+// launch.  A chunk is 32 tokens, two groups of 16; a page holds 16 or more, so that a group lies in one.  Lane (token r16 of a
+// group, quarter qd of the head) loads its quarter row with one load of D / 8 bytes, and the scale with it; next chunk's loads are
+// on their way while one computes.
 //   S^T[token][head] = K Q^T: the quarter row, widened, is the operand of D / 32 MFMAs as it is -- their contraction takes the
 //                      head's elements in the order (quarter, 8 of it, next 8 ..), and so does q's operand
 //   O^T[d][head]    += V^T P^T: the widened rows go through LDS, where the transposing reads make columns of them; the
@@ -265,15 +266,15 @@ static void kv4_decode_dispatch(const Kv4Decode& a, int waves, DecodeLeast least
 
 // Waves per workgroup (ops/__init__.py has the same numbers, and chooses Z by them).  us, 8 kv heads of 128 unless said, one
 // launch or, with ->, two:
-//   fewer than 64 pairs leave CUs free for slices, and four waves meet sooner than eight: 1 x 128 4.9 (eight 5.7), 1 x 2000 eight slices
-//     -> 7.6 (9.1), 4 x 1000 -> 8.3 (8.9);
-//   up to 512 eight waves take the place of slices: 32 x 2000 16.5 (four 20.5, four and two slices -> 21.1), 33 x 1001 of 12 heads of
-//     64 10.5 (10.8, -> 13.5);
-//   from 512 on the LDS of eight (two workgroups per CU) makes short contexts wait: 64 x 512 10.8 (11.3), 64 x 8192 96.6 (97.2);
-//   from 1024 on two: 128 x 1000 27.6 (one 31.1, four 27.9), 160 x 1000 34.0 (36.9, 36.1), 128 x 4000 94.1 (99.9, 96.0), 100 x 1000 of
-//     12 heads of 64 22.5 (27.2, 22.9), 128 x 300 12.8 (12.8, 13.6); a short context pays for it, 128 x 60 7.8 (6.1, 8.0);
-//   from 1536 on a wave has a pair to itself: 256 x 60 8.0 (two 10.7, four 13.4), 256 x 640 34.0 (35.0, 38.8), 200 x 1000 42.7
-//     (43.4, 43.3), 250 x 500 of 12 heads of 64 25.4 (28.6, 30.9), 130 x 1000 of them 28.9 (28.9, 29.9).
+//   fewer than 64 pairs leave CUs free for slices, and four waves meet sooner than eight: 1 x 128 4.9 (eight 5.9), 1 x 2000 eight slices
+//     -> 7.6 (9.2), 4 x 1000 -> 8.3 (9.7);
+//   up to 512 eight waves take the place of slices: 32 x 2000 16.7 (four 18.2, four and two slices -> 21.8), 33 x 1001 of 12 heads of
+//     64 10.4 (10.5, -> 12.2);
+//   from 512 on the LDS of eight (two workgroups per CU) makes short contexts wait: 64 x 512 10.5 (11.1), 64 x 8192 96.2 (97.0);
+//   from 1024 on two: 128 x 1000 27.2 (one 29.2, four 27.7), 160 x 1000 33.4 (35.7, 36.4), 128 x 4000 93.1 (99.4, 95.6), 100 x 1000 of
+//     12 heads of 64 22.3 (26.5, 22.9), 128 x 300 12.6 (12.5, 13.6); a short context pays for it, 128 x 60 7.5 (6.1, 7.8);
+//   from 1536 on a wave has a pair to itself: 256 x 60 7.9 (two 10.6, four 13.6), 256 x 640 33.5 (34.8, 38.6), 200 x 1000 42.3
+//     (43.1, 43.2), 250 x 500 of 12 heads of 64 25.6 (27.3, 30.7), 130 x 1000 of them 28.3 (28.3, 29.7).
 static int kv4_decode_waves(int64_t pairs) { return pairs >= 1536 ? 1 : pairs >= 1024 ? 2 : pairs >= 512 ? 4 : pairs >= 64 ? 8 : 4; }
 
 void launch_kv4_decode(int dtype, const Kv4Decode& a, float scale, hipStream_t s) {

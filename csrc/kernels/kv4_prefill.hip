@@ -12,7 +12,7 @@
 // Z > 1: few rows after long contexts leave CUs idle, so that Z workgroups share an item's tiles; each leaves its rows' maximum,
 // sum and unnormalised result, which kv4_prefill_merge_kernel joins.
 //
-// 4 x 4096 rows of 32 / 8 heads of 128 take 514 us (1.04 PFLOP/s; a large matrix product reaches 1.40): the matrix cores work in half
+// 4 x 4096 rows of 32 / 8 heads of 128 take 508 us (1.05 PFLOP/s; a large matrix product reaches 1.40): the matrix cores work in half
 // of a CU's busy cycles at 2.0 GHz, vector instructions issue in 48 %, a wave's own products and softmax one after the other.  Scores of the
 // next tile beside this one's softmax need 32 registers more, which the compiler takes from elsewhere: with 64 keys at a time
 // they spill (1320 us), with 32 keys it is 678 us, and 760 with the order prescribed.

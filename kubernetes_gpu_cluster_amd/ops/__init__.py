@@ -388,7 +388,7 @@ def prefill_work_list(query_lens: list[int], seq_lens: list[int]) -> tuple[list[
 def kv4_prefill_slices(rows: int, seqs: int, num_heads: int, num_kv_heads: int, head_dim: int, max_len: int) -> int:
     """Workgroups that share the keys of each item of a prompt step over a 4-bit cache (csrc/kernels/kv4_prefill.hip): as
     many as give each CU two of them (three with heads of 64), with four tiles of 64 keys or more each.  One -> several,
-    us: 3 x 301 after 7000, 12 heads of 64, 113 -> 40 (eight); 8 kv heads of 128, 300 after 2000 54 -> 36, 20 after 8000 171 -> 23,
+    us: 3 x 301 after 7000, 12 heads of 64, 113 -> 42 (seven); 8 kv heads of 128, 300 after 2000 54 -> 36, 20 after 8000 171 -> 23,
     16 x 30 after 1000 41 -> 34, 1000 after 4000 110 -> 98.  The merge takes 4 to 8 us, so that short prompts have one: 512
     17.4 -> 26."""
     tiles = math.ceil(max_len / 64)
