@@ -270,7 +270,7 @@ void rope_kv_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor q_out, T
               "q_out bf16 / fp16");
   const kgc::RopeAxes ax = rope_axes(positions, sections, cos_sin, T, d, use_rope);
   TORCH_CHECK(slot_mapping.scalar_type() == at::kLong && slot_mapping.numel() == T, "slot_mapping int64 [T]");
-  TORCH_CHECK(slot_mapping.is_contiguous() && (ax.n || positions.is_contiguous()), "positions, slot_mapping contiguous");
+  TORCH_CHECK(slot_mapping.is_contiguous() && (ax.n || !use_rope || positions.is_contiguous()), "positions, slot_mapping contiguous");
   TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() && cos_sin.size(1) == d,
               "cos_sin fp32 [max_pos, d]");
   if ((kv4 || ax.n) && q_norm_w.has_value()) {
@@ -278,7 +278,7 @@ void rope_kv_write(Tensor qkv, Tensor positions, Tensor cos_sin, Tensor q_out, T
     for (const Tensor* t : {&*q_norm_w, &*k_norm_w}) {
       TORCH_CHECK(t->scalar_type() == q_out.scalar_type() && t->is_contiguous(), "qk norm weights in q's dtype");
       check_same_dev(qkv, *t, "qk norm weights");
-      aligned16(*t, "qk norm weights");
+      if (kv4) aligned16(*t, "qk norm weights");
     }
   }
   // an empty q_out: write k / v only (prefill_attention_rope rotates q as it loads it)

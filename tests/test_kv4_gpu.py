@@ -1032,3 +1032,19 @@ def test_axes_leave_out_slots_beyond_the_pool(gpu, cache, T, slices):
         got.append([q, k_all.float(), v_all.float()])
     assert all(torch.equal(a, b) for a, b in zip(*got))
     assert got[0][1].any() and not got[1][1][nb:].any() and not got[1][2][nb:].any()
+
+
+@pytest.mark.parametrize("cache", ["auto", "fp4"])
+def test_strided_positions_that_nothing_reads(gpu, cache):
+    """Without rotation positions may lie anywhere: the call writes what it writes with dense ones."""
+    d, T, bf = 64, 8, torch.bfloat16
+    x = torch.randn(T, 4 * d, device=gpu).to(bf)
+    table, pos, slots = ref.rope_cos_sin_cache(d, 20, 10000.0).to(gpu), torch.arange(2 * T, device=gpu), torch.arange(T, device=gpu)
+    got = []
+    for p in (pos[::2], pos[:T]):
+        if cache == "fp4":
+            kc, vc = (torch.zeros(ops.kv4_cache_shape(2, 1, 16, d), dtype=torch.uint8, device=gpu) for _ in range(2))
+        else:
+            kc, vc = torch.zeros(2, 1, 16, d, device=gpu).to(bf), torch.zeros(2, 1, 2, d, 8, device=gpu).to(bf)
+        got.append([ops.rope_kv_write(x, p, table, kc, vc, slots, 2, 1, d, use_rope=False), kc, vc])
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and got[0][1].any()
